@@ -100,6 +100,13 @@ SYMBOLS = [
     ("acehip_mod_up", C.c_int, [_vp, _vp, _vp, _u32, _u32, _vp]),
     ("acehip_bsgs_inner", C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _vp]),
     ("acehip_bsgs_inner_rot", C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _vp]),
+    # operators of a transformer on ciphertexts
+    ("acehip_linear_i8", C.c_int, [_vp, _vp, _vp, _vp, C.c_size_t, _u32, _u32, _u32, _u32, _vp, _vp, C.c_size_t, _u32, _u32, _u32, _vp]),
+    ("acehip_rope_messages", C.c_int, [_vp, _vp, _vp, C.c_size_t, _vp, C.c_size_t, _u32, _vp, _vp, _u32, _u32, _vp]),
+    ("acehip_rope", C.c_int, [_vp, _vp, _vp, _vp, _vp, C.c_size_t, C.c_size_t, _u32, _u32, _u32, _u32, C.c_int, _u32, _u32, _u32, _vp]),
+    ("acehip_linattn_scores", C.c_int, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, C.c_int, _u32, _u32, _u32, _vp]),
+    ("acehip_linattn_out", C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _vp, _vp, C.c_int, _u32, _u32, _u32, _vp]),
+    ("acehip_linattn_state", C.c_int, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _vp, _vp, _u32, _u32, _u32, _vp]),
     ("acehip_shard_create", _vp, [_vp, _u32, _u32]),
     ("acehip_shard_destroy", None, [_vp]),
     ("acehip_shard_num_q", _u32, [_vp, _u32]),
@@ -171,6 +178,12 @@ def load_library(path=None):
 class HwOp(C.Structure):
     """acehip_hw_op of include/acehip.h"""
     _fields_ = [("op", C.c_uint32), ("prime_gi", C.c_uint32), ("res", C.c_void_p), ("a", C.c_void_p), ("b", C.c_void_p)]
+
+
+class Mat(C.Structure):
+    """acehip_mat of include/acehip.h"""
+    _fields_ = [("data", C.c_void_p), ("head_stride", C.c_size_t), ("row_stride", C.c_size_t), ("col_stride", C.c_size_t),
+                ("comp_stride", C.c_size_t)]
 
 
 class HwRange(C.Structure):
@@ -392,3 +405,40 @@ class AceHip:
         for d in (da, dk, d0, d1):
             d.free()
         return o0, o1
+
+    # ---- operators of a transformer on ciphertexts: device addresses in, launched on `stream` ----
+    def mat(self, ptr, head=0, row=0, col=0, comp=0):
+        """matrix of ciphertexts at device address ptr, strides in words"""
+        return Mat(ptr, head, row, col, comp)
+
+    def linear_i8(self, out, x, d_w, ld_w, rows, n_in, n_out, n_comp, level, pos0=0, n_limbs=None, d_mul=None, d_tok=None, tok_stride=0, stream=None):
+        self.check(self.lib.acehip_linear_i8(self.h, _ref(out), _ref(x), d_w, ld_w, rows, n_in, n_out, n_comp, d_mul, d_tok, tok_stride, level, pos0,
+                                             level - pos0 if n_limbs is None else n_limbs, stream))
+
+    def rope_messages(self, d_cos, d_sin, out_stride, d_pos, pos_stride, n_pos, freq, axis, n_axes, stream=None):
+        n = len(freq)
+        if len(axis) != n:
+            raise ValueError("as many axes as frequencies are needed")
+        self.check(self.lib.acehip_rope_messages(self.h, d_cos, d_sin, out_stride, d_pos, pos_stride, n_pos, (C.c_double * n)(*freq), (_u32 * n)(*axis), n,
+                                                 n_axes, stream))
+
+    def rope(self, out, x, d_cos, d_sin, pair_stride, row_stride, n_heads, rows, dim, n_comp, level, pos0=0, n_limbs=None, interleaved=False, stream=None):
+        self.check(self.lib.acehip_rope(self.h, _ref(out), _ref(x), d_cos, d_sin, pair_stride, row_stride, n_heads, rows, dim, n_comp, interleaved, level,
+                                        pos0, level - pos0 if n_limbs is None else n_limbs, stream))
+
+    def linattn_scores(self, p3, q, k, n_heads, n_kv_heads, n_q, n_k, dim, level, pos0=0, n_limbs=None, causal=True, stream=None):
+        self.check(self.lib.acehip_linattn_scores(self.h, _ref(p3), _ref(q), _ref(k), n_heads, n_kv_heads, n_q, n_k, dim, causal, level, pos0,
+                                                  level - pos0 if n_limbs is None else n_limbs, stream))
+
+    def linattn_out(self, o3, q, state, p, v, n_heads, n_kv_heads, n_q, n_k, dim_k, dim_v, level, pos0=0, n_limbs=None, d_in=None, d_decay=None, causal=True,
+                    stream=None):
+        self.check(self.lib.acehip_linattn_out(self.h, _ref(o3), _ref(q), _ref(state), _ref(p), _ref(v), n_heads, n_kv_heads, n_q, n_k, dim_k, dim_v, d_in,
+                                               d_decay, causal, level, pos0, level - pos0 if n_limbs is None else n_limbs, stream))
+
+    def linattn_state(self, s3, state, k, v, n_heads, n_kv_heads, n_k, dim_k, dim_v, level, pos0=0, n_limbs=None, d_keep=None, d_decay=None, stream=None):
+        self.check(self.lib.acehip_linattn_state(self.h, _ref(s3), _ref(state), _ref(k), _ref(v), n_heads, n_kv_heads, n_k, dim_k, dim_v, d_keep, d_decay,
+                                                 level, pos0, level - pos0 if n_limbs is None else n_limbs, stream))
+
+
+def _ref(m):
+    return None if m is None else C.byref(m)

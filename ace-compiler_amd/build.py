@@ -25,7 +25,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 OBJDIR = os.path.join(LIBDIR, "obj")
 LIB = os.path.join(LIBDIR, "libacehip.so")
-SOURCES = ["kernels.hip", "ntt_fast.hip", "keyswitch.hip", "rt_kernels.hip", "embed.hip", "hw_batch.hip", "shard.hip", "api_core.cpp", "api_hw_batch.cpp", "api_ops.cpp", "api_shard.cpp", "host_params.cpp"]
+SOURCES = ["kernels.hip", "ntt_fast.hip", "keyswitch.hip", "rt_kernels.hip", "embed.hip", "hw_batch.hip", "shard.hip", "linear.hip", "rope.hip", "linattn.hip", "api_core.cpp", "api_hw_batch.cpp", "api_ops.cpp", "api_shard.cpp", "api_nn.cpp", "host_params.cpp"]
 # every header / include file of csrc/ (an object is rebuilt when ANY of them changes: cheaper than tracking who includes what)
 HEADERS = sorted(n for n in os.listdir(CSRC) if n.endswith((".hpp", ".inc"))) + [os.path.join("..", "..", "include", "acehip.h")]
 ROCM_LIB = "/opt/rocm/lib"

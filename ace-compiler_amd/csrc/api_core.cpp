@@ -47,7 +47,8 @@ u32 replica_chunk() {
   return v;
 }
 static const char* const kStatName[ST_COUNT] = {"ntt", "elementwise", "rotate", "decomp_modup", "key_inner_product",
-                                                "mod_down", "rescale", "key_switch", "encode", "zero_fill_executed", "elementwise_mul", "ntt_launched"};
+                                                "mod_down", "rescale", "key_switch", "encode", "zero_fill_executed", "elementwise_mul", "ntt_launched",
+                                                "linear_i8", "rope", "linear_attention"};
 
 extern "C" {
 

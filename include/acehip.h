@@ -235,7 +235,8 @@ int acehip_key_switch(acehip_ctx* ctx, uint64_t* d_out0, uint64_t* d_out1, const
  * fills that were actually executed, i.e. not proven dead inside their batch, and "elementwise_mul", the limb-ops that contain a
  * modular multiplication (units = limb multiplications): what a CPU spends its elementwise time on); and "ntt_launched": every
  * limb-transform the library launched, the ones inside the pipelines (ModUp, ModDown, Rescale, key-switch, encode) included -- "ntt"
- * only counts the direct entry points (units = limb-transforms, bytes = 16 per coefficient index: multiply by N). */
+ * only counts the direct entry points (units = limb-transforms, bytes = 16 per coefficient index: multiply by N).  "linear_i8", "rope",
+ * "linear_attention": the operators on ciphertexts further down (units = result ciphertexts). */
 typedef struct acehip_stat {
   uint64_t calls, units, bytes;
 } acehip_stat;
@@ -339,6 +340,71 @@ int acehip_bsgs_inner(acehip_ctx* ctx, uint64_t* const* d_out0, uint64_t* const*
 int acehip_bsgs_inner_rot(acehip_ctx* ctx, uint64_t* const* d_out0, uint64_t* const* d_out1, const uint64_t* const* d_in0,
                           const uint64_t* const* d_in1, const uint32_t* h_in_auto, const uint64_t* const* d_pt, uint32_t g, uint32_t b,
                           uint32_t pt_q_limbs, uint32_t level, acehip_stream stream);
+
+/* ---- operators of a transformer on ciphertexts (no reference counterpart) ----
+ * Softmax-free transformer layers in the data's own form.  Feature i of a matrix of tokens is one ciphertext: tokens (or the sequences of a
+ * batch) lie in its slots, further tokens in further rows.  All operands are residues in the NTT domain, limb positions [pos0, pos0 + n_limbs)
+ * of polynomials extended at `level`; the limb at position pos of a polynomial is at its start + pos*N, as everywhere in this header.  Results
+ * are the canonical residues of the formulas, exact: scales multiply, nothing is rescaled (acehip_rescale2) or relinearised
+ * (acehip_key_switch on the third polynomial) inside.
+ *
+ * A matrix of ciphertexts, strides in words: polynomial `comp` of element (head, row, col) starts at data + head*head_stride + row*row_stride
+ * + col*col_stride + comp*comp_stride.  The strides of an operand are arbitrary (0: the same for all); the polynomials of a result must not
+ * overlap each other or an operand, unless an entry point says so.  Of every polynomial only the limbs of the call are touched.  Counts of
+ * zero are allowed: an empty result is nothing to do, an empty sum is zero.
+ * Integer factors (`int64_t`, device arrays, shared by all limbs) are taken mod each prime: llround(factor * scaling_factor) is the usual value.
+ * Data, weights and factors are read when the launch runs; arrays named h_* are read during the call.  Under a replica selection, operands in the
+ * arena follow their replica, and the result has to lie in the arena; a sharded context computes the limbs that it owns. */
+typedef struct acehip_mat {
+  uint64_t* data;
+  size_t    head_stride, row_stride, col_stride, comp_stride;
+} acehip_mat;
+
+/* Linear layer with int8 weights, a factor for each output channel and a plaintext for each row of tokens:
+ *   out[r][j] = tok[r] (*) mul[j] * sum_{i < n_in} w[j][i] in[r][i]      for each of the n_comp polynomials of the ciphertexts
+ * in: rows x n_in, out: rows x n_out (head_stride unused).  d_w: [n_out][ld_w] bytes, ld_w >= n_in, no alignment asked.  d_mul: [n_out] or NULL.
+ * d_tok: plaintext polynomial of row r (encoded scales of its tokens: 0 / 1 masks padding) at d_tok + r*tok_stride, or NULL. */
+#define ACEHIP_LINEAR_MAX_IN 65536
+int acehip_linear_i8(acehip_ctx* ctx, const acehip_mat* out, const acehip_mat* in, const int8_t* d_w, size_t ld_w, uint32_t rows, uint32_t n_in,
+                     uint32_t n_out, uint32_t n_comp, const int64_t* d_mul, const uint64_t* d_tok, size_t tok_stride, uint32_t level, uint32_t pos0,
+                     uint32_t n_limbs, acehip_stream stream);
+
+/* Rotary positions with several axes (time, height, width ...): pair i of features turns by pos[axis[i]][t] * freq[i] at token t.
+ * acehip_rope_messages writes the messages of the tables, d_cos / d_sin[i*out_stride + t] for i < n_pairs, t < n_pos, as doubles
+ * (acehip_encode[_batch] kind 1 makes plaintexts of them).  d_pos: [n_axes][pos_stride] doubles; h_freq, h_axis: HOST arrays of n_pairs,
+ * axis indices below n_axes <= 8.  The angle is the rounded product of the two doubles. */
+int acehip_rope_messages(acehip_ctx* ctx, double* d_cos, double* d_sin, size_t out_stride, const double* d_pos, size_t pos_stride, uint32_t n_pos,
+                         const double* h_freq, const uint32_t* h_axis, uint32_t n_pairs, uint32_t n_axes, acehip_stream stream);
+/* acehip_rope turns the encrypted features: of pair i < dim/2 of every head and row,
+ *   out0 = in0 (*) cos[row][i] - in1 (*) sin[row][i],   out1 = in0 (*) sin[row][i] + in1 (*) cos[row][i]
+ * with the features (i, i + dim/2), or (2i, 2i + 1) if `interleaved`, as columns of the matrices.  The plaintext of (row, i) is at
+ * d_cos / d_sin + row*row_stride + i*pair_stride; heads and polynomials share it.  out may be in itself (same address and strides). */
+int acehip_rope(acehip_ctx* ctx, const acehip_mat* out, const acehip_mat* in, const uint64_t* d_cos, const uint64_t* d_sin, size_t pair_stride,
+                size_t row_stride, uint32_t n_heads, uint32_t rows, uint32_t dim, uint32_t n_comp, int interleaved, uint32_t level, uint32_t pos0,
+                uint32_t n_limbs, acehip_stream stream);
+
+/* Linear attention with a decay for each head.  (x) is the product of two ciphertexts before relinearisation, (a0, a1) (x) (b0, b1) =
+ * (a0 b0, a0 b1 + a1 b0, a1 b1): operands have two polynomials, results three.  Head h reads the keys and values of head
+ * h' = h / (n_heads / n_kv_heads).  Rows of q, key, v are tokens, columns features.
+ * A chunk of a prompt: scores (relinearise, rescale), out with the state so far, state.  One token (recurrent form): state with n_k = 1
+ * (relinearise, rescale), then out with n_q = 1 and no scores.
+ *
+ * p3[h][t][s] = sum_a q[t][h][a] (x) key[s][h'][a].  causal: of query t only the keys s <= t + n_k - n_q, the other results are not written.
+ * (matrices q and key: element (head, row = token, col = feature)) */
+int acehip_linattn_scores(acehip_ctx* ctx, const acehip_mat* p3, const acehip_mat* q, const acehip_mat* key, uint32_t n_heads, uint32_t n_kv_heads,
+                          uint32_t n_q, uint32_t n_k, uint32_t dim, int causal, uint32_t level, uint32_t pos0, uint32_t n_limbs, acehip_stream stream);
+/* o3[h][t][b] = in[h][t] * sum_{a < dim_k} q[t][h][a] (x) state[h][a][b] + sum_s decay[h][t + n_k - n_q - s] * p[h][t][s] (x) v[s][h'][b]
+ * q and state, p and v may be NULL (both of a pair): that sum is empty.  causal: s <= t + n_k - n_q, the other p are not read; otherwise all
+ * s < n_k, and d_decay is NULL.  d_in: [n_heads][n_q], d_decay: [n_heads][n_k] by distance; NULL: 1. */
+int acehip_linattn_out(acehip_ctx* ctx, const acehip_mat* o3, const acehip_mat* q, const acehip_mat* state, const acehip_mat* p, const acehip_mat* v,
+                       uint32_t n_heads, uint32_t n_kv_heads, uint32_t n_q, uint32_t n_k, uint32_t dim_k, uint32_t dim_v, const int64_t* d_in,
+                       const int64_t* d_decay, int causal, uint32_t level, uint32_t pos0, uint32_t n_limbs, acehip_stream stream);
+/* s3[h][a][b] = keep[h] * state[h][a][b] + sum_{s < n_k} decay[h][n_k - 1 - s] * key[s][h'][a] (x) v[s][h'][b]
+ * state may be NULL (nothing kept).  d_keep: [n_heads], d_decay: [n_heads][n_k] by distance; NULL: 1.  s3 may be state itself (same address and
+ * strides: its polynomials 0 and 1 are replaced). */
+int acehip_linattn_state(acehip_ctx* ctx, const acehip_mat* s3, const acehip_mat* state, const acehip_mat* key, const acehip_mat* v, uint32_t n_heads,
+                         uint32_t n_kv_heads, uint32_t n_k, uint32_t dim_k, uint32_t dim_v, const int64_t* d_keep, const int64_t* d_decay, uint32_t level,
+                         uint32_t pos0, uint32_t n_limbs, acehip_stream stream);
 
 /* Debug aid: with enable != 0 the pipeline entry points (acehip_key_switch, acehip_modup_digits[_to], acehip_mod_down[2],
  * acehip_rescale[2], acehip_encode[_batch]) record every range of CALLER memory they read or write (device pointer, words);
