@@ -160,6 +160,8 @@ int acehip_linear_i8(acehip_ctx* c, const acehip_mat* out, const acehip_mat* in,
   a.tok_stride = tok_stride;
   a.rows = rows, a.n_in = n_in, a.n_out = n_out, a.n_comp = n_comp;
   a.level = level, a.pos0 = pos0, a.n_limbs = n_limbs;
+  a.wide_primes = true;
+  for (u32 p = pos0; p < pos0 + n_limbs; ++p) a.wide_primes = a.wide_primes && c->hp.q(limb_prime(p, level, c->hp.L)) >> 32;
   for (const DevCtx& dc : launch_dcs(c)) launch_linear_i8(dc, a, (hipStream_t)s);
   const u64 limb = 8ull * c->hp.N * n_limbs * rows;
   stat(ST_LINEAR, (u64)rows * n_out, limb * ((u64)n_comp * n_in + (u64)n_comp * n_out + (d_tok ? 1 : 0)) + (u64)n_in * n_out);

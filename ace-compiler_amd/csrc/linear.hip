@@ -3,8 +3,239 @@
 
 namespace acehip {
 
-// One coefficient per lane, kJ outputs: residues split at 31 bits, so that each half times a weight is one multiply-add into a signed
-// 64-bit sum (|sum| <= 2^31 * 2^7 * 2^16 inputs).
+// ------------------------------------------------------------------------------------------------
+// Matrix-core form.  For one limb the layer is a product of an int8 matrix W by a matrix X of residues, columns = coefficients.  A residue is
+// NP signed bytes d_p (x = sum d_p 256^p: the bytes of (x + C) ^ C, C = 0x80 in every byte), so
+//   sum_i w_ji x_i = sum_p 256^p (W D_p)_j ,
+// NP int8 matrix products with exact 32-bit sums (|sum| <= 2^14 * 2^16 inputs), joined in 64-bit parts and reduced once.
+// Layout: a workgroup of four waves takes 16 WN columns and 16 MT WJ outputs, WJ waves along the outputs and WN = 4 / WJ along the columns.  A step
+// is 64 inputs: the residues are read once by the workgroup, their bytes transposed in registers (four inputs of a column by v_perm_b32) and left in
+// LDS as the B fragments of v_mfma_i32_16x16x64_i8 (1 KiB each, read without bank conflicts); the weights' rows are the A fragments as they lie
+// in memory.  Residues are requested two steps ahead, weights one.
+// ------------------------------------------------------------------------------------------------
+typedef int v4i_t __attribute__((ext_vector_type(4)));
+typedef int v4i_any_t __attribute__((ext_vector_type(4), aligned(1)));
+// global address space spelled out: FLAT loads would count as LDS accesses too, and every wait for LDS would wait for them
+#define GLOBAL __attribute__((address_space(1)))
+template <class T>
+__device__ __forceinline__ GLOBAL T* global(T* p) { return (GLOBAL T*)(uintptr_t)p; }
+constexpr u64 kBytes7 = 0x7f7f7f7f7f7f7full;  // the largest residue of seven signed bytes
+
+__device__ __forceinline__ u32 perm(u32 hi, u32 lo, u32 sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
+// bytes of four dwords transposed: o[b] = byte b of l[0..3]
+__device__ __forceinline__ void transpose4(const u32 (&l)[4], u32 (&o)[4]) {
+  const u32 a01 = perm(l[1], l[0], 0x05010400u), a23 = perm(l[3], l[2], 0x05010400u);
+  const u32 b01 = perm(l[1], l[0], 0x07030602u), b23 = perm(l[3], l[2], 0x07030602u);
+  o[0] = perm(a23, a01, 0x05040100u);
+  o[1] = perm(a23, a01, 0x07060302u);
+  o[2] = perm(b23, b01, 0x05040100u);
+  o[3] = perm(b23, b01, 0x07060302u);
+}
+// LDS writes of the workgroup are visible, loads from memory stay in flight
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+template <int NP, int MT, int WJ>
+__device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a, v4i_t* frag, const DevPrime& P, u32 rep, u32 pos, u32 row, u32 comp, u32 n0, u32 j0) {
+  constexpr int WN = 4 / WJ;
+  const u32 t = threadIdx.x, lane = t & 63u, wave = t >> 6;
+  const u32 wj = wave % WJ, wn = wave / WJ;
+  const u64 off = (u64)pos * c.N + n0;
+  const u64 xs = a.in.col;
+  const GLOBAL u64* x = global(reb(c, a.in.d, rep) + row * a.in.row + comp * a.in.comp + off + (t & 15u));
+  const u32 k4 = t >> 4;  // this thread stages inputs 4 k4 .. 4 k4 + 3 of a step
+  const GLOBAL int8_t* w = global(reb(c, a.w, rep));
+  const u64 w_end = (u64)(a.n_out - 1) * a.ld_w + a.n_in;
+  const u32 kg = 16 * (lane >> 4);
+  u64 w_row[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) w_row[m] = (u64)min(j0 + (wj * MT + m) * 16 + (lane & 15u), a.n_out - 1) * a.ld_w + kg;
+  const u32 full = a.n_in / 64;  // steps that need no guard
+
+  struct Raw {
+    u64 v[WN][4];
+  };
+  auto load_x = [&](u32 s, Raw& r) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const GLOBAL u64* p = x + (u64)(s * 64 + 4 * k4 + i) * xs;
+#pragma unroll
+      for (int u = 0; u < WN; ++u) r.v[u][i] = p[u * 16];
+    }
+  };
+  auto stage = [&](const Raw& r, v4i_t* buf) {
+    constexpr u64 C = NP == 8 ? 0x8080808080808080ull : 0x80808080808080ull;
+#pragma unroll
+    for (int u = 0; u < WN; ++u) {
+      u32 lo[4], hi[4], o[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const u64 v = r.v[u][i] + C;
+        lo[i] = (u32)v ^ (u32)C;
+        hi[i] = (u32)(v >> 32) ^ (u32)(C >> 32);
+      }
+      transpose4(lo, *(u32(*)[4])o);
+      transpose4(hi, *(u32(*)[4])(o + 4));
+      u32* d = (u32*)(buf + u * NP * 64) + ((k4 >> 2) * 16 + (t & 15u)) * 4 + (k4 & 3u);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) d[p * 256] = o[p];
+    }
+  };
+  auto load_w = [&](u32 s, v4i_t (&aw)[MT]) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) aw[m] = *(const GLOBAL v4i_any_t*)(w + w_row[m] + s * 64);
+  };
+
+  v4i_t acc[MT][NP];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int p = 0; p < NP; ++p) acc[m][p] = v4i_t{0, 0, 0, 0};
+  auto multiply = [&](const v4i_t (&aw)[MT], const v4i_t* buf) {
+    const v4i_t* b = buf + wn * NP * 64 + lane;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const v4i_t bp = b[p * 64];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) acc[m][p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(aw[m], bp, acc[m][p], 0, 0, 0);
+    }
+  };
+  v4i_t *buf0 = frag, *buf1 = frag + WN * NP * 64;
+  if (full) {
+    Raw raw0, raw1;
+    v4i_t aw0[MT], aw1[MT];
+    load_x(0, raw0);
+    load_w(0, aw0);
+    load_x(min(1u, full - 1), raw1);
+    stage(raw0, buf0);
+    load_x(min(2u, full - 1), raw0);
+    u32 s = 0;
+    // a step: the next one's fragments are staged while this one's are multiplied (requests past the last step repeat it)
+    for (; s + 2 < full; s += 2) {
+      lds_barrier();
+      load_w(s + 1, aw1);
+      stage(raw1, buf1);
+      load_x(min(s + 3, full - 1), raw1);
+      multiply(aw0, buf0);
+      lds_barrier();
+      load_w(s + 2, aw0);
+      stage(raw0, buf0);
+      load_x(min(s + 4, full - 1), raw0);
+      multiply(aw1, buf1);
+    }
+    lds_barrier();
+    if (s + 2 == full) {
+      load_w(s + 1, aw1);
+      stage(raw1, buf1);
+      multiply(aw0, buf0);
+      lds_barrier();
+      multiply(aw1, buf1);
+    } else {
+      multiply(aw0, buf0);
+    }
+  }
+  if (a.n_in % 64) {  // the last inputs: those past n_in are zero, and their weights may be any, only not past the array
+    Raw r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const u32 k = full * 64 + 4 * k4 + i;
+      const GLOBAL u64* p = x + (u64)min(k, a.n_in - 1) * xs;
+#pragma unroll
+      for (int u = 0; u < WN; ++u) {
+        const u64 v = p[u * 16];
+        r.v[u][i] = k < a.n_in ? v : 0;
+      }
+    }
+    v4i_t aw[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        u32 v = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v |= (u32)(uint8_t)w[min(w_row[m] + full * 64 + 4 * d + i, w_end - 1)] << (8 * i);
+        aw[m][d] = (int)v;
+      }
+    lds_barrier();  // the last full step has been read
+    stage(r, buf0);
+    lds_barrier();
+    multiply(aw, buf0);
+  }
+
+  // lane: column lane % 16, outputs 4 (lane / 16) + r of each tile.  The value is lo + 2^32 hi, |lo|, |hi| < 2^56:
+  //   2^32 (hi + 2^57) by its companion floor(2^96 / q) -> below 2q, and lo + bias with bias = 2^57 - (2^57 + 2^89) mod q + q; their sum is below 2^63
+  const u64 q = P.q, mh = P.prec128_hi;
+  const u32 n = wn * 16 + (lane & 15u);
+  GLOBAL u64* y = global(reb(c, a.out.d, rep) + row * a.out.row + comp * a.out.comp + off + n);
+  const u64 tok = a.tok ? global(reb(c, a.tok, rep))[row * a.tok_stride + off + n] : 0;
+  const u64 c32p = (mh << 32) | (P.prec128_lo >> 32);
+  const u64 bias = (1ull << 57) + q - add_mod(signed_mod(1ll << 57, q, mh), mul_shoup(1ull << 57, 1ull << 32, c32p, q), q);
+  int weight[4] = {1, 1 << 8, 1 << 16, 1 << 24};
+  asm volatile("" : "+s"(weight[0]), "+s"(weight[1]), "+s"(weight[2]), "+s"(weight[3]));  // opaque: each byte's sum joins by ONE v_mad_i64_i32
+  ulong2* factor = (ulong2*)frag;  // channel factors and their companions (at most one too small: products below 3q)
+  if (a.mul) {
+    lds_barrier();
+    if (t < 16 * MT * WJ) {
+      const u64 m = signed_mod(global(reb(c, a.mul, rep))[min(j0 + t, a.n_out - 1)], q, mh);
+      factor[t] = ulong2{m, m * mh + mulhi64(m, P.prec128_lo)};
+    }
+    lds_barrier();
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const u32 jl = (wj * MT + m) * 16 + 4 * (lane >> 4) + r;
+      int64_t lo = (int64_t)bias, hi = 1ll << 57;
+#pragma unroll
+      for (int p = 0; p < 4; ++p) lo += (int64_t)acc[m][p][r] * weight[p];
+#pragma unroll
+      for (int p = 4; p < NP; ++p) hi += (int64_t)acc[m][p][r] * weight[p - 4];
+      const u64 s = ((u64)hi << 32) - mulhi64((u64)hi, c32p) * q + (u64)lo;
+      u64 v;
+      if (a.mul) {
+        const ulong2 f = factor[jl];
+        v = s * f.x - mulhi64(s, f.y) * q;
+        v = v >= 2 * q ? v - 2 * q : v;
+      } else {
+        v = s - mulhi64(s, mh) * q;
+      }
+      v = v >= q ? v - q : v;
+      if (a.tok) v = mul_mod(v, tok, P);
+      if (j0 + jl < a.n_out) y[(j0 + jl) * a.out.col] = v;
+    }
+}
+
+template <int MT, int WJ>
+__global__ __launch_bounds__(256, 2) void linear_i8_mfma_kernel(DevCtx c, LinearArgs a, u32 j_blocks, u32 n_blocks) {
+  __shared__ v4i_t frag[2 * (4 / WJ) * 8 * 64];
+  // workgroups that read the same columns run side by side on one XCD (ids congruent mod 8): its L2 keeps the residues for all outputs
+  const u32 cols = gridDim.x / j_blocks;
+  u32 jb, cb;
+  if ((cols & 7u) == 0) {
+    const u32 b = blockIdx.x >> 3;
+    jb = b % j_blocks;
+    cb = (b / j_blocks) * 8 + (blockIdx.x & 7u);
+  } else {
+    jb = blockIdx.x % j_blocks;
+    cb = blockIdx.x / j_blocks;
+  }
+  jb = __builtin_amdgcn_readfirstlane(jb);
+  cb = __builtin_amdgcn_readfirstlane(cb);
+  const u32 pos = a.pos0 + blockIdx.y, gi = limb_prime(pos, a.level, c.L), rep = c.rep0 + blockIdx.z;
+  if (!owns(c, gi)) return;
+  const DevPrime P = c.primes[gi];
+  const u32 nb = cb % n_blocks, rc = cb / n_blocks, comp = rc % a.n_comp, row = rc / a.n_comp;
+  const u32 n0 = nb * (64 / WJ), j0 = jb * (16 * MT * WJ);
+  if (P.q <= kBytes7) linear_tile<7, MT, WJ>(c, a, frag, P, rep, pos, row, comp, n0, j0);
+  else                linear_tile<8, MT, WJ>(c, a, frag, P, rep, pos, row, comp, n0, j0);
+}
+
+// Rings below 64 and primes below 2^32: one coefficient per lane, kJ outputs: residues split at 31 bits, so that each half times a weight is one multiply-add into a
+// signed 64-bit sum (|sum| <= 2^31 * 2^7 * 2^16 inputs).
 constexpr u32 kJ = 8;
 __global__ __launch_bounds__(256) void linear_i8_kernel(DevCtx c, LinearArgs a, u32 n_blocks, u32 j_blocks) {
   u32 b = blockIdx.x;
@@ -44,9 +275,27 @@ __global__ __launch_bounds__(256) void linear_i8_kernel(DevCtx c, LinearArgs a, 
   }
 }
 
+template <int MT, int WJ>
+static void launch_mfma(const DevCtx& c, const LinearArgs& a, hipStream_t s) {
+  const u32 n_blocks = c.N / (64 / WJ), j_blocks = (a.n_out + 16 * MT * WJ - 1) / (16 * MT * WJ);
+  hipLaunchKernelGGL((linear_i8_mfma_kernel<MT, WJ>), dim3(n_blocks * j_blocks * a.n_comp * a.rows, a.n_limbs, c.nrep), dim3(256), 0, s, c, a, j_blocks, n_blocks);
+}
+
 void launch_linear_i8(const DevCtx& c, const LinearArgs& a, hipStream_t s) {
-  const u32 n_blocks = (c.N + 255) / 256, j_blocks = (a.n_out + kJ - 1) / kJ;
-  hipLaunchKernelGGL(linear_i8_kernel, dim3(n_blocks * j_blocks * a.n_comp * a.rows, a.n_limbs, c.nrep), dim3(256), 0, s, c, a, n_blocks, j_blocks);
+  if (c.N < 64 || !a.wide_primes) {
+    const u32 n_blocks = (c.N + 255) / 256, j_blocks = (a.n_out + kJ - 1) / kJ;
+    hipLaunchKernelGGL(linear_i8_kernel, dim3(n_blocks * j_blocks * a.n_comp * a.rows, a.n_limbs, c.nrep), dim3(256), 0, s, c, a, n_blocks, j_blocks);
+  } else if (a.n_out <= 16) {
+    launch_mfma<1, 1>(c, a, s);
+  } else if (a.n_out <= 32) {
+    launch_mfma<2, 1>(c, a, s);
+  } else if (a.n_out <= 64) {
+    launch_mfma<4, 1>(c, a, s);
+  } else if (a.n_out <= 128) {
+    launch_mfma<4, 2>(c, a, s);
+  } else {
+    launch_mfma<4, 4>(c, a, s);
+  }
 }
 
 }  // namespace acehip

@@ -28,6 +28,7 @@ struct LinearArgs {
   const u64* tok;      // plaintext polynomial of row r at tok + r*tok_stride, or null
   u64 tok_stride;
   u32 rows, n_in, n_out, n_comp, level, pos0, n_limbs;
+  bool wide_primes;    // every prime of the call is above 2^32
 };
 void launch_linear_i8(const DevCtx& c, const LinearArgs& a, hipStream_t s);
 
