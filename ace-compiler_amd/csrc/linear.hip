@@ -1,4 +1,6 @@
 // linear.hip -- int8 linear layers on ciphertexts: y_j = tok * mul_j * sum_i w_ji x_i mod q on every limb and coefficient.
+#include <type_traits>
+
 #include "nn.hpp"
 
 namespace acehip {
@@ -22,6 +24,12 @@ __device__ __forceinline__ GLOBAL T* global(T* p) { return (GLOBAL T*)(uintptr_t
 constexpr u64 kBytes7 = 0x7f7f7f7f7f7f7full;  // the largest residue of seven signed bytes
 
 __device__ __forceinline__ u32 perm(u32 hi, u32 lo, u32 sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
+// a pointer that is the same for the wave, kept on the scalar unit
+template <class T>
+__device__ __forceinline__ T* uniform(T* p) {
+  const u64 v = (u64)p;
+  return (T*)(((u64)(u32)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) | (u32)__builtin_amdgcn_readfirstlane((int)v));
+}
 // bytes of four dwords transposed: o[b] = byte b of l[0..3]
 __device__ __forceinline__ void transpose4(const u32 (&l)[4], u32 (&o)[4]) {
   const u32 a01 = perm(l[1], l[0], 0x05010400u), a23 = perm(l[3], l[2], 0x05010400u);
@@ -41,30 +49,34 @@ __device__ __forceinline__ void lds_barrier() {
 template <int NP, int MT, int WJ>
 __device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a, v4i_t* frag, const DevPrime& P, u32 rep, u32 pos, u32 row, u32 comp, u32 n0, u32 j0) {
   constexpr int WN = 4 / WJ;
-  const u32 t = threadIdx.x, lane = t & 63u, wave = t >> 6;
+  const u32 t = threadIdx.x, lane = t & 63u, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const u32 wj = wave % WJ, wn = wave / WJ;
   const u64 off = (u64)pos * c.N + n0;
+  const u32 last = (a.n_in - 1) / 64;  // step (n_in > 0)
+  // addresses: a uniform 64-bit base that moves with the step plus 32-bit offsets of the lanes that stay (linear_fits)
   const u64 xs = a.in.col;
-  const GLOBAL u64* x = global(reb(c, a.in.d, rep) + row * a.in.row + comp * a.in.comp + off + (t & 15u));
+  const u64* x = uniform(reb(c, a.in.d, rep) + row * a.in.row + comp * a.in.comp + off);
   const u32 k4 = t >> 4;  // this thread stages inputs 4 k4 .. 4 k4 + 3 of a step
-  const GLOBAL int8_t* w = global(reb(c, a.w, rep));
-  const u64 w_end = (u64)(a.n_out - 1) * a.ld_w + a.n_in;
-  const u32 kg = 16 * (lane >> 4);
-  u64 w_row[MT];
+  u32 x_at[4];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) w_row[m] = (u64)min(j0 + (wj * MT + m) * 16 + (lane & 15u), a.n_out - 1) * a.ld_w + kg;
-  const u32 full = a.n_in / 64;  // steps that need no guard
+  for (int i = 0; i < 4; ++i) x_at[i] = 8 * ((4 * k4 + i) * (u32)xs + (t & 15u));
+  const GLOBAL char* w = (const GLOBAL char*)global(uniform(reb(c, a.w, rep) + (u64)j0 * a.ld_w));
+  const u32 kg = 16 * (lane >> 4);
+  u32 w_at[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) w_at[m] = min((wj * MT + m) * 16 + (lane & 15u), a.n_out - 1 - j0) * (u32)a.ld_w + kg;
 
   struct Raw {
     u64 v[WN][4];
   };
+  // a step's inputs through a buffer descriptor that ends behind the last of them: those past n_in read as zero
   auto load_x = [&](u32 s, Raw& r) {
+    const u32 there = min(a.n_in - min(s * 64, a.n_in), 64u);
+    const auto d = __builtin_amdgcn_make_buffer_rsrc((void*)uniform(x + (u64)s * 64 * xs), 0, __builtin_amdgcn_readfirstlane((int)(there * (u32)xs * 8)), 0x00027000);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const GLOBAL u64* p = x + (u64)(s * 64 + 4 * k4 + i) * xs;
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int u = 0; u < WN; ++u) r.v[u][i] = p[u * 16];
-    }
+      for (int u = 0; u < WN; ++u) r.v[u][i] = __builtin_bit_cast(u64, __builtin_amdgcn_raw_buffer_load_b64(d, (int)x_at[i] + u * 128, 0, 0));
   };
   auto stage = [&](const Raw& r, v4i_t* buf) {
     constexpr u64 C = NP == 8 ? 0x8080808080808080ull : 0x80808080808080ull;
@@ -86,7 +98,26 @@ __device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a
   };
   auto load_w = [&](u32 s, v4i_t (&aw)[MT]) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m) aw[m] = *(const GLOBAL v4i_any_t*)(w + w_row[m] + s * 64);
+    for (int m = 0; m < MT; ++m) {
+      u32 at = w_at[m];
+      asm("" : "+v"(at));  // (opaque: the loads stay one uniform base and a 32-bit offset each, not a running 64-bit pointer per lane)
+      aw[m] = *(const GLOBAL v4i_any_t*)(w + s * 64 + at);
+    }
+  };
+  // the last step's (s = last; a function of s, so that nothing of it is kept over the loop): nothing is read past the array, and the weights
+  // past n_in may be any
+  auto load_w_last = [&](u32 s, v4i_t (&aw)[MT]) {
+    if (a.n_in - 64 * s == 64) return load_w(s, aw);
+    const u64 end = (u64)(a.n_out - 1 - j0) * a.ld_w + a.n_in - 64 * s;  // of the array, seen from this step
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      u32 at = w_at[m];
+      asm volatile("" : "+v"(at));
+      const int64_t from = at + 16ull <= end ? (int64_t)at : (int64_t)end - 16;  // (may lie before this step: the array has 16 bytes)
+      const u32 skip = 8 * (u32)min((int64_t)at - from, (int64_t)15);
+      unsigned __int128 v = __builtin_bit_cast(unsigned __int128, (v4i_t) * (const GLOBAL v4i_any_t*)(w + s * 64 + from));
+      aw[m] = __builtin_bit_cast(v4i_t, v >> skip);
+    }
   };
 
   v4i_t acc[MT][NP];
@@ -104,72 +135,42 @@ __device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a
     }
   };
   v4i_t *buf0 = frag, *buf1 = frag + WN * NP * 64;
-  if (full) {
+  {
     Raw raw0, raw1;
     v4i_t aw0[MT], aw1[MT];
     load_x(0, raw0);
-    load_w(0, aw0);
-    load_x(min(1u, full - 1), raw1);
+    load_x(1, raw1);
+    if (last == 0) load_w_last(0, aw0);
+    else           load_w(0, aw0);
     stage(raw0, buf0);
-    load_x(min(2u, full - 1), raw0);
-    u32 s = 0;
+    load_x(2, raw0);
     // a step: the next one's fragments are staged while this one's are multiplied (requests past the last step repeat it)
-    for (; s + 2 < full; s += 2) {
+    auto next = [&](u32 s, Raw& raw, v4i_t (&aw)[MT], v4i_t* buf) {
+      if (s > last) return;
+      if (s == last) load_w_last(s, aw);
+      else           load_w(s, aw);
+      stage(raw, buf);
+      load_x(s + 2, raw);
+    };
+    for (u32 s = 0;; s += 2) {
       lds_barrier();
-      load_w(s + 1, aw1);
-      stage(raw1, buf1);
-      load_x(min(s + 3, full - 1), raw1);
+      next(s + 1, raw1, aw1, buf1);
       multiply(aw0, buf0);
+      if (s + 1 > last) break;
       lds_barrier();
-      load_w(s + 2, aw0);
-      stage(raw0, buf0);
-      load_x(min(s + 4, full - 1), raw0);
+      next(s + 2, raw0, aw0, buf0);
       multiply(aw1, buf1);
+      if (s + 2 > last) break;
     }
-    lds_barrier();
-    if (s + 2 == full) {
-      load_w(s + 1, aw1);
-      stage(raw1, buf1);
-      multiply(aw0, buf0);
-      lds_barrier();
-      multiply(aw1, buf1);
-    } else {
-      multiply(aw0, buf0);
-    }
-  }
-  if (a.n_in % 64) {  // the last inputs: those past n_in are zero, and their weights may be any, only not past the array
-    Raw r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const u32 k = full * 64 + 4 * k4 + i;
-      const GLOBAL u64* p = x + (u64)min(k, a.n_in - 1) * xs;
-#pragma unroll
-      for (int u = 0; u < WN; ++u) {
-        const u64 v = p[u * 16];
-        r.v[u][i] = k < a.n_in ? v : 0;
-      }
-    }
-    v4i_t aw[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        u32 v = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v |= (u32)(uint8_t)w[min(w_row[m] + full * 64 + 4 * d + i, w_end - 1)] << (8 * i);
-        aw[m][d] = (int)v;
-      }
-    lds_barrier();  // the last full step has been read
-    stage(r, buf0);
-    lds_barrier();
-    multiply(aw, buf0);
   }
 
   // lane: column lane % 16, outputs 4 (lane / 16) + r of each tile.  The value is lo + 2^32 hi, |lo|, |hi| < 2^56:
   //   2^32 (hi + 2^57) by its companion floor(2^96 / q) -> below 2q, and lo + bias with bias = 2^57 - (2^57 + 2^89) mod q + q; their sum is below 2^63
   const u64 q = P.q, mh = P.prec128_hi;
-  const u32 n = wn * 16 + (lane & 15u);
-  GLOBAL u64* y = global(reb(c, a.out.d, rep) + row * a.out.row + comp * a.out.comp + off + n);
+  const u32 n = wn * 16 + (lane & 15u), g4 = 4 * (lane >> 4);
+  GLOBAL char* y = (GLOBAL char*)global(uniform(reb(c, a.out.d, rep) + row * a.out.row + comp * a.out.comp + off + (u64)(j0 + wj * MT * 16) * a.out.col));
+  const u32 y_at = 8 * (g4 * (u32)a.out.col + n);
+  const u32 left = a.n_out - j0 - min(a.n_out - j0, wj * MT * 16);  // outputs of this wave that are there
   const u64 tok = a.tok ? global(reb(c, a.tok, rep))[row * a.tok_stride + off + n] : 0;
   const u64 c32p = (mh << 32) | (P.prec128_lo >> 32);
   const u64 bias = (1ull << 57) + q - add_mod(signed_mod(1ll << 57, q, mh), mul_shoup(1ull << 57, 1ull << 32, c32p, q), q);
@@ -184,29 +185,34 @@ __device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a
     }
     lds_barrier();
   }
+  auto finish = [&](auto with_mul, auto with_tok) {
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const u32 jl = (wj * MT + m) * 16 + 4 * (lane >> 4) + r;
-      int64_t lo = (int64_t)bias, hi = 1ll << 57;
+      for (int r = 0; r < 4; ++r) {
+        int64_t lo = (int64_t)bias, hi = 1ll << 57;
 #pragma unroll
-      for (int p = 0; p < 4; ++p) lo += (int64_t)acc[m][p][r] * weight[p];
+        for (int p = 0; p < 4; ++p) lo += (int64_t)acc[m][p][r] * weight[p];
 #pragma unroll
-      for (int p = 4; p < NP; ++p) hi += (int64_t)acc[m][p][r] * weight[p - 4];
-      const u64 s = ((u64)hi << 32) - mulhi64((u64)hi, c32p) * q + (u64)lo;
-      u64 v;
-      if (a.mul) {
-        const ulong2 f = factor[jl];
-        v = s * f.x - mulhi64(s, f.y) * q;
-        v = v >= 2 * q ? v - 2 * q : v;
-      } else {
-        v = s - mulhi64(s, mh) * q;
+        for (int p = 4; p < NP; ++p) hi += (int64_t)acc[m][p][r] * weight[p - 4];
+        const u64 s = ((u64)hi << 32) - mulhi64((u64)hi, c32p) * q + (u64)lo;
+        u64 v;
+        if (with_mul) {
+          const ulong2 f = factor[(wj * MT + m) * 16 + g4 + r];
+          v = s * f.x - mulhi64(s, f.y) * q;
+          v = v >= 2 * q ? v - 2 * q : v;
+        } else {
+          v = s - mulhi64(s, mh) * q;
+        }
+        v = v >= q ? v - q : v;
+        if (with_tok) v = mul_mod(v, tok, P);
+        if (m * 16 + r + g4 < left) *(GLOBAL u64*)(y + (u64)(m * 16 + r) * a.out.col * 8 + y_at) = v;
       }
-      v = v >= q ? v - q : v;
-      if (a.tok) v = mul_mod(v, tok, P);
-      if (j0 + jl < a.n_out) y[(j0 + jl) * a.out.col] = v;
-    }
+  };
+  using T = std::true_type;
+  using F = std::false_type;
+  if (a.mul) a.tok ? finish(T{}, T{}) : finish(T{}, F{});
+  else       a.tok ? finish(F{}, T{}) : finish(F{}, F{});
 }
 
 template <int MT, int WJ>
@@ -234,7 +240,7 @@ __global__ __launch_bounds__(256, 2) void linear_i8_mfma_kernel(DevCtx c, Linear
   else                linear_tile<8, MT, WJ>(c, a, frag, P, rep, pos, row, comp, n0, j0);
 }
 
-// Rings below 64 and primes below 2^32: one coefficient per lane, kJ outputs: residues split at 31 bits, so that each half times a weight is one multiply-add into a
+// What the matrix-core form does not take (linear_fits: rings below 64, primes below 2^32, strides of over 32 MiB): one coefficient per lane, kJ outputs: residues split at 31 bits, so that each half times a weight is one multiply-add into a
 // signed 64-bit sum (|sum| <= 2^31 * 2^7 * 2^16 inputs).
 constexpr u32 kJ = 8;
 __global__ __launch_bounds__(256) void linear_i8_kernel(DevCtx c, LinearArgs a, u32 n_blocks, u32 j_blocks) {
@@ -275,6 +281,12 @@ __global__ __launch_bounds__(256) void linear_i8_kernel(DevCtx c, LinearArgs a, 
   }
 }
 
+// the matrix-core form: rings and primes that it takes, lane offsets below 2^32, and an array of weights that holds a fragment of 16 bytes
+static bool linear_fits(const DevCtx& c, const LinearArgs& a) {
+  return c.N >= 64 && a.wide_primes && a.in.col <= (1u << 22) && a.out.col <= (1u << 23) && a.ld_w <= (1u << 24) && a.n_in != 0 &&
+         (u64)(a.n_out - 1) * a.ld_w + a.n_in >= 16;
+}
+
 template <int MT, int WJ>
 static void launch_mfma(const DevCtx& c, const LinearArgs& a, hipStream_t s) {
   const u32 n_blocks = c.N / (64 / WJ), j_blocks = (a.n_out + 16 * MT * WJ - 1) / (16 * MT * WJ);
@@ -282,7 +294,7 @@ static void launch_mfma(const DevCtx& c, const LinearArgs& a, hipStream_t s) {
 }
 
 void launch_linear_i8(const DevCtx& c, const LinearArgs& a, hipStream_t s) {
-  if (c.N < 64 || !a.wide_primes) {
+  if (!linear_fits(c, a)) {
     const u32 n_blocks = (c.N + 255) / 256, j_blocks = (a.n_out + kJ - 1) / kJ;
     hipLaunchKernelGGL(linear_i8_kernel, dim3(n_blocks * j_blocks * a.n_comp * a.rows, a.n_limbs, c.nrep), dim3(256), 0, s, c, a, n_blocks, j_blocks);
   } else if (a.n_out <= 16) {
