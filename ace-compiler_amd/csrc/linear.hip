@@ -46,7 +46,36 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-template <int NP, int MT, int WJ>
+// Weights as A fragments, [tile of 16 outputs][step][lane] of 16 bytes, zero past the matrix.  In memory a fragment's lanes read 16 bytes from each of
+// 16 rows, which costs the L1 cache 64 look-ups (four waves a fragment long: the product waits for them); packed, a fragment is 1 KiB in a row.
+__global__ __launch_bounds__(256) void linear_pack_kernel(const int8_t* w, u64 ld_w, u32 n_in, u32 n_out, u32 steps, u32 n_frags, v4i_t* out) {
+  const u32 f = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63u;
+  if (f >= n_frags) return;
+  const u32 j = (f / steps) * 16 + (lane & 15u), k = (f % steps) * 64 + 16 * (lane >> 4);
+  v4i_t v{0, 0, 0, 0};
+  if (j < n_out && k < n_in) {
+    const GLOBAL int8_t* p = global(w) + j * ld_w + k;
+    if (k + 16 <= n_in) {
+      v = *(const GLOBAL v4i_any_t*)p;
+    } else {
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (k + 4 * d + i < n_in) v[d] |= (int)((u32)(uint8_t)p[4 * d + i] << (8 * i));
+    }
+  }
+  out[(u64)f * 64 + lane] = v;
+}
+
+// a * w mod q up to multiples of q for a < 2^63, with nq = -q and a companion wp of w that is at most two units of 2^-64 too small: below 4q
+// (the quotient leaves out the low product and two carries: at most 3 too small, and a w / q - a wp / 2^64 < 1)
+__device__ __forceinline__ u64 mul_near(u64 a, u64 w, u64 wp, u64 nq) {
+  const u64 h = (u64)(u32)(a >> 32) * (u32)(wp >> 32) + __umulhi((u32)(a >> 32), (u32)wp) + __umulhi((u32)a, (u32)(wp >> 32));
+  return a * w + h * nq;
+}
+
+template <int NP, int MT, int WJ, bool PACKED>
 __device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a, v4i_t* frag, const DevPrime& P, u32 rep, u32 pos, u32 row, u32 comp, u32 n0, u32 j0) {
   constexpr int WN = 4 / WJ;
   const u32 t = threadIdx.x, lane = t & 63u, wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -60,19 +89,20 @@ __device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a
   u32 x_at[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) x_at[i] = 8 * ((4 * k4 + i) * (u32)xs + (t & 15u));
-  const GLOBAL char* w = (const GLOBAL char*)global(uniform(reb(c, a.w, rep) + (u64)j0 * a.ld_w));
-  const u32 kg = 16 * (lane >> 4);
-  u32 w_at[MT];
+  const GLOBAL char* w = (const GLOBAL char*)global(uniform(PACKED ? (const int8_t*)a.packed : reb(c, a.w, rep) + (u64)j0 * a.ld_w));
+  u32 w_at[MT];  // of the lane's row; packed: of the fragments' tile, in steps
 #pragma unroll
-  for (int m = 0; m < MT; ++m) w_at[m] = min((wj * MT + m) * 16 + (lane & 15u), a.n_out - 1 - j0) * (u32)a.ld_w + kg;
+  for (int m = 0; m < MT; ++m)
+    w_at[m] = PACKED ? min(j0 / 16 + wj * MT + m, (a.n_out - 1) / 16) * (last + 1)
+                     : min((wj * MT + m) * 16 + (lane & 15u), a.n_out - 1 - j0) * (u32)a.ld_w + 16 * (lane >> 4);
 
   struct Raw {
     u64 v[WN][4];
   };
   // a step's inputs through a buffer descriptor that ends behind the last of them: those past n_in read as zero
   auto load_x = [&](u32 s, Raw& r) {
-    const u32 there = min(a.n_in - min(s * 64, a.n_in), 64u);
-    const auto d = __builtin_amdgcn_make_buffer_rsrc((void*)uniform(x + (u64)s * 64 * xs), 0, __builtin_amdgcn_readfirstlane((int)(there * (u32)xs * 8)), 0x00027000);
+    const int there = max(min((int)a.n_in - (int)s * 64, 64), 0);
+    const auto d = __builtin_amdgcn_make_buffer_rsrc((void*)uniform(x + (u64)s * 64 * xs), 0, __builtin_amdgcn_readfirstlane(there * (int)xs * 8), 0x00027000);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -99,15 +129,16 @@ __device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a
   auto load_w = [&](u32 s, v4i_t (&aw)[MT]) {
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      u32 at = w_at[m];
+      u32 at = PACKED ? lane * 16 : w_at[m];
       asm("" : "+v"(at));  // (opaque: the loads stay one uniform base and a 32-bit offset each, not a running 64-bit pointer per lane)
-      aw[m] = *(const GLOBAL v4i_any_t*)(w + s * 64 + at);
+      if (PACKED) aw[m] = *(const GLOBAL v4i_t*)(w + (u64)(w_at[m] + s) * 1024 + at);
+      else        aw[m] = *(const GLOBAL v4i_any_t*)(w + s * 64 + at);
     }
   };
   // the last step's (s = last; a function of s, so that nothing of it is kept over the loop): nothing is read past the array, and the weights
   // past n_in may be any
   auto load_w_last = [&](u32 s, v4i_t (&aw)[MT]) {
-    if (a.n_in - 64 * s == 64) return load_w(s, aw);
+    if (PACKED || a.n_in - 64 * s == 64) return load_w(s, aw);
     const u64 end = (u64)(a.n_out - 1 - j0) * a.ld_w + a.n_in - 64 * s;  // of the array, seen from this step
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
@@ -144,11 +175,12 @@ __device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a
     else           load_w(0, aw0);
     stage(raw0, buf0);
     load_x(2, raw0);
-    // a step: the next one's fragments are staged while this one's are multiplied (requests past the last step repeat it)
+    // a step: the next one's fragments are staged while this one's are multiplied.  Past the last step weights are read again and inputs as
+    // zeros, never to be used: without a branch around the requests the compiler counts them exactly and waits for the oldest only
     auto next = [&](u32 s, Raw& raw, v4i_t (&aw)[MT], v4i_t* buf) {
-      if (s > last) return;
-      if (s == last) load_w_last(s, aw);
-      else           load_w(s, aw);
+      if (!PACKED && s >= last) load_w_last(last, aw);
+      else                      load_w(min(s, last), aw);
+      __builtin_amdgcn_sched_barrier(0);  // (weights first: the next step waits for them and not for the inputs behind them)
       stage(raw, buf);
       load_x(s + 2, raw);
     };
@@ -164,19 +196,23 @@ __device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a
     }
   }
 
-  // lane: column lane % 16, outputs 4 (lane / 16) + r of each tile.  The value is lo + 2^32 hi, |lo|, |hi| < 2^56:
-  //   2^32 (hi + 2^57) by its companion floor(2^96 / q) -> below 2q, and lo + bias with bias = 2^57 - (2^57 + 2^89) mod q + q; their sum is below 2^63
+  // lane: column lane % 16, outputs 4 (lane / 16) + r of each tile.  V = sum_p acc_p 256^p is reduced by its rounded quotient in floating point:
+  // |V / q| <= 2^7 n_in <= 2^23, and what the doubles leave out of V (its low 32 bits, roundings of two units of 2^32) is below 2^-6 q at primes
+  // above 2^40.  V - round(V / q) q is then within (1/2 + 2^-5) q of zero, so its low 64 bits tell it.
   const u64 q = P.q, mh = P.prec128_hi;
   const u32 n = wn * 16 + (lane & 15u), g4 = 4 * (lane >> 4);
   GLOBAL char* y = (GLOBAL char*)global(uniform(reb(c, a.out.d, rep) + row * a.out.row + comp * a.out.comp + off + (u64)(j0 + wj * MT * 16) * a.out.col));
   const u32 y_at = 8 * (g4 * (u32)a.out.col + n);
   const u32 left = a.n_out - j0 - min(a.n_out - j0, wj * MT * 16);  // outputs of this wave that are there
   const u64 tok = a.tok ? global(reb(c, a.tok, rep))[row * a.tok_stride + off + n] : 0;
-  const u64 c32p = (mh << 32) | (P.prec128_lo >> 32);
-  const u64 bias = (1ull << 57) + q - add_mod(signed_mod(1ll << 57, q, mh), mul_shoup(1ull << 57, 1ull << 32, c32p, q), q);
+  const u64 tokp = tok * mh + mulhi64(tok, P.prec128_lo), nq = 0 - q;
+  const double inv = 4294967296.0 / (double)q;
+  double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the rounded integer, plus those of the constant
+  u64 start = __builtin_bit_cast(u64, magic) * q;
+  asm volatile("" : "+s"(magic), "+s"(start));
   int weight[4] = {1, 1 << 8, 1 << 16, 1 << 24};
   asm volatile("" : "+s"(weight[0]), "+s"(weight[1]), "+s"(weight[2]), "+s"(weight[3]));  // opaque: each byte's sum joins by ONE v_mad_i64_i32
-  ulong2* factor = (ulong2*)frag;  // channel factors and their companions (at most one too small: products below 3q)
+  ulong2* factor = (ulong2*)frag;  // channel factors and their companions
   if (a.mul) {
     lds_barrier();
     if (t < 16 * MT * WJ) {
@@ -190,22 +226,31 @@ __device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        int64_t lo = (int64_t)bias, hi = 1ll << 57;
+        int64_t lo = 0;
 #pragma unroll
         for (int p = 0; p < 4; ++p) lo += (int64_t)acc[m][p][r] * weight[p];
+        u32 hi = 0;
+        double f = 0;
 #pragma unroll
-        for (int p = 4; p < NP; ++p) hi += (int64_t)acc[m][p][r] * weight[p - 4];
-        const u64 s = ((u64)hi << 32) - mulhi64((u64)hi, c32p) * q + (u64)lo;
-        u64 v;
-        if (with_mul) {
-          const ulong2 f = factor[(wj * MT + m) * 16 + g4 + r];
-          v = s * f.x - mulhi64(s, f.y) * q;
-          v = v >= 2 * q ? v - 2 * q : v;
-        } else {
-          v = s - mulhi64(s, mh) * q;
+        for (int p = NP - 1; p >= 4; --p) {
+          hi = (hi << 8) + (u32)acc[m][p][r];
+          f = __builtin_fma(f, 256.0, (double)acc[m][p][r]);
         }
-        v = v >= q ? v - q : v;
-        if (with_tok) v = mul_mod(v, tok, P);
+        f += (double)(int)(lo >> 32);
+        const u64 quot = __builtin_bit_cast(u64, __builtin_fma(f, inv, magic));
+        u64 v = (u64)lo + ((u64)hi << 32) + start + quot * nq;
+        if (with_mul || with_tok) {
+          v += q;
+          if (with_mul) {
+            const ulong2 f = factor[(wj * MT + m) * 16 + g4 + r];
+            v = mul_near(v, f.x, f.y, nq);
+          }
+          if (with_tok) v = mul_near(v, tok, tokp, nq);
+          v = v >= 2 * q ? v - 2 * q : v;
+          v = v >= q ? v - q : v;
+        } else {
+          v += q & (u64)((int64_t)v >> 63);
+        }
         if (m * 16 + r + g4 < left) *(GLOBAL u64*)(y + (u64)(m * 16 + r) * a.out.col * 8 + y_at) = v;
       }
   };
@@ -215,7 +260,7 @@ __device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a
   else       a.tok ? finish(F{}, T{}) : finish(F{}, F{});
 }
 
-template <int MT, int WJ>
+template <int MT, int WJ, bool PACKED>
 __global__ __launch_bounds__(256, 2) void linear_i8_mfma_kernel(DevCtx c, LinearArgs a, u32 j_blocks, u32 n_blocks) {
   __shared__ v4i_t frag[2 * (4 / WJ) * 8 * 64];
   // workgroups that read the same columns run side by side on one XCD (ids congruent mod 8): its L2 keeps the residues for all outputs
@@ -236,11 +281,11 @@ __global__ __launch_bounds__(256, 2) void linear_i8_mfma_kernel(DevCtx c, Linear
   const DevPrime P = c.primes[gi];
   const u32 nb = cb % n_blocks, rc = cb / n_blocks, comp = rc % a.n_comp, row = rc / a.n_comp;
   const u32 n0 = nb * (64 / WJ), j0 = jb * (16 * MT * WJ);
-  if (P.q <= kBytes7) linear_tile<7, MT, WJ>(c, a, frag, P, rep, pos, row, comp, n0, j0);
-  else                linear_tile<8, MT, WJ>(c, a, frag, P, rep, pos, row, comp, n0, j0);
+  if (P.q <= kBytes7) linear_tile<7, MT, WJ, PACKED>(c, a, frag, P, rep, pos, row, comp, n0, j0);
+  else                linear_tile<8, MT, WJ, PACKED>(c, a, frag, P, rep, pos, row, comp, n0, j0);
 }
 
-// What the matrix-core form does not take (linear_fits: rings below 64, primes below 2^32, strides of over 32 MiB): one coefficient per lane, kJ outputs: residues split at 31 bits, so that each half times a weight is one multiply-add into a
+// What the matrix-core form does not take (linear_fits: rings below 64, primes below 2^40, strides of over 32 MiB): one coefficient per lane, kJ outputs: residues split at 31 bits, so that each half times a weight is one multiply-add into a
 // signed 64-bit sum (|sum| <= 2^31 * 2^7 * 2^16 inputs).
 constexpr u32 kJ = 8;
 __global__ __launch_bounds__(256) void linear_i8_kernel(DevCtx c, LinearArgs a, u32 n_blocks, u32 j_blocks) {
@@ -290,7 +335,21 @@ static bool linear_fits(const DevCtx& c, const LinearArgs& a) {
 template <int MT, int WJ>
 static void launch_mfma(const DevCtx& c, const LinearArgs& a, hipStream_t s) {
   const u32 n_blocks = c.N / (64 / WJ), j_blocks = (a.n_out + 16 * MT * WJ - 1) / (16 * MT * WJ);
-  hipLaunchKernelGGL((linear_i8_mfma_kernel<MT, WJ>), dim3(n_blocks * j_blocks * a.n_comp * a.rows, a.n_limbs, c.nrep), dim3(256), 0, s, c, a, j_blocks, n_blocks);
+  const dim3 grid(n_blocks * j_blocks * a.n_comp * a.rows, a.n_limbs, c.nrep);
+  if (a.packed) hipLaunchKernelGGL((linear_i8_mfma_kernel<MT, WJ, true>), grid, dim3(256), 0, s, c, a, j_blocks, n_blocks);
+  else          hipLaunchKernelGGL((linear_i8_mfma_kernel<MT, WJ, false>), grid, dim3(256), 0, s, c, a, j_blocks, n_blocks);
+}
+
+// Outputs whose packed weights fit the workspace at a time (all of them unless the layer is large); 0: the weights are read as they lie
+u32 linear_pack_outputs(const DevCtx& c, const LinearArgs& a, size_t ws_bytes) {
+  if (!linear_fits(c, a) || a.n_out <= 32) return 0;
+  const u64 tile = (u64)((a.n_in + 63) / 64) * 1024, tiles = ws_bytes / tile;
+  if (tiles * 16 >= a.n_out) return a.n_out;
+  return (u32)(tiles / 16 * 256);  // whole workgroups
+}
+void launch_linear_pack(const LinearArgs& a, void* out, hipStream_t s) {
+  const u32 steps = (a.n_in + 63) / 64, n_frags = (a.n_out + 15) / 16 * steps;
+  hipLaunchKernelGGL(linear_pack_kernel, dim3((n_frags + 3) / 4), dim3(256), 0, s, a.w, a.ld_w, a.n_in, a.n_out, steps, n_frags, (v4i_t*)out);
 }
 
 void launch_linear_i8(const DevCtx& c, const LinearArgs& a, hipStream_t s) {

@@ -28,8 +28,11 @@ struct LinearArgs {
   const u64* tok;      // plaintext polynomial of row r at tok + r*tok_stride, or null
   u64 tok_stride;
   u32 rows, n_in, n_out, n_comp, level, pos0, n_limbs;
-  bool wide_primes;    // every prime of the call is above 2^32
+  bool wide_primes;    // every prime of the call is above 2^40
+  const void* packed = nullptr;  // the weights as launch_linear_pack left them
 };
+u32 linear_pack_outputs(const DevCtx& c, const LinearArgs& a, size_t ws_bytes);
+void launch_linear_pack(const LinearArgs& a, void* out, hipStream_t s);
 void launch_linear_i8(const DevCtx& c, const LinearArgs& a, hipStream_t s);
 
 // cos and sin of pos[axis[i]][t] * freq[i] (rope.hip)
