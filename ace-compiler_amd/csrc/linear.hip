@@ -1,4 +1,5 @@
 // linear.hip -- int8 linear layers on ciphertexts: y_j = tok * mul_j * sum_i w_ji x_i mod q on every limb and coefficient.
+#include <algorithm>
 #include <type_traits>
 
 #include "nn.hpp"
@@ -75,9 +76,9 @@ __device__ __forceinline__ u64 mul_near(u64 a, u64 w, u64 wp, u64 nq) {
   return a * w + h * nq;
 }
 
-template <int NP, int MT, int WJ, bool PACKED>
+template <int NP, int MT, int WJ, int WN, bool PACKED>
 __device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a, v4i_t* frag, const DevPrime& P, u32 rep, u32 pos, u32 row, u32 comp, u32 n0, u32 j0) {
-  constexpr int WN = 4 / WJ;
+  constexpr int G = 4 / WJ;  // column blocks that a thread stages
   const u32 t = threadIdx.x, lane = t & 63u, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const u32 wj = wave % WJ, wn = wave / WJ;
   const u64 off = (u64)pos * c.N + n0;
@@ -85,10 +86,10 @@ __device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a
   // addresses: a uniform 64-bit base that moves with the step plus 32-bit offsets of the lanes that stay (linear_fits)
   const u64 xs = a.in.col;
   const u64* x = uniform(reb(c, a.in.d, rep) + row * a.in.row + comp * a.in.comp + off);
-  const u32 k4 = t >> 4;  // this thread stages inputs 4 k4 .. 4 k4 + 3 of a step
+  const u32 k4 = (t >> 4) & 15u, u0 = t >> 8;  // this thread stages inputs 4 k4 .. 4 k4 + 3 of a step in column blocks u0, u0 + WN / G ..
   u32 x_at[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x_at[i] = 8 * ((4 * k4 + i) * (u32)xs + (t & 15u));
+  for (int i = 0; i < 4; ++i) x_at[i] = 8 * ((4 * k4 + i) * (u32)xs + u0 * 16 + (t & 15u));
   const GLOBAL char* w = (const GLOBAL char*)global(uniform(PACKED ? (const int8_t*)a.packed : reb(c, a.w, rep) + (u64)j0 * a.ld_w));
   u32 w_at[MT];  // of the lane's row; packed: of the fragments' tile, in steps
 #pragma unroll
@@ -97,7 +98,7 @@ __device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a
                      : min((wj * MT + m) * 16 + (lane & 15u), a.n_out - 1 - j0) * (u32)a.ld_w + 16 * (lane >> 4);
 
   struct Raw {
-    u64 v[WN][4];
+    u64 v[G][4];
   };
   // a step's inputs through a buffer descriptor that ends behind the last of them: those past n_in read as zero
   auto load_x = [&](u32 s, Raw& r) {
@@ -106,12 +107,12 @@ __device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int u = 0; u < WN; ++u) r.v[u][i] = __builtin_bit_cast(u64, __builtin_amdgcn_raw_buffer_load_b64(d, (int)x_at[i] + u * 128, 0, 0));
+      for (int u = 0; u < G; ++u) r.v[u][i] = __builtin_bit_cast(u64, __builtin_amdgcn_raw_buffer_load_b64(d, (int)x_at[i] + u * (WN / G * 128), 0, 0));
   };
   auto stage = [&](const Raw& r, v4i_t* buf) {
     constexpr u64 C = NP == 8 ? 0x8080808080808080ull : 0x80808080808080ull;
 #pragma unroll
-    for (int u = 0; u < WN; ++u) {
+    for (int u = 0; u < G; ++u) {
       u32 lo[4], hi[4], o[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -121,18 +122,22 @@ __device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a
       }
       transpose4(lo, *(u32(*)[4])o);
       transpose4(hi, *(u32(*)[4])(o + 4));
-      u32* d = (u32*)(buf + u * NP * 64) + ((k4 >> 2) * 16 + (t & 15u)) * 4 + (k4 & 3u);
+      u32* d = (u32*)(buf + (u0 + u * (WN / G)) * NP * 64) + ((k4 >> 2) * 16 + (t & 15u)) * 4 + (k4 & 3u);
 #pragma unroll
       for (int p = 0; p < NP; ++p) d[p * 256] = o[p];
     }
   };
+  const auto packed = __builtin_amdgcn_make_buffer_rsrc((void*)uniform(a.packed), 0, PACKED ? (int)((a.n_out + 15) / 16 * (last + 1) * 1024) : 0, 0x00027000);
   auto load_w = [&](u32 s, v4i_t (&aw)[MT]) {
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      u32 at = PACKED ? lane * 16 : w_at[m];
-      asm("" : "+v"(at));  // (opaque: the loads stay one uniform base and a 32-bit offset each, not a running 64-bit pointer per lane)
-      if (PACKED) aw[m] = *(const GLOBAL v4i_t*)(w + (u64)(w_at[m] + s) * 1024 + at);
-      else        aw[m] = *(const GLOBAL v4i_any_t*)(w + s * 64 + at);
+      if (PACKED) {
+        aw[m] = __builtin_bit_cast(v4i_t, __builtin_amdgcn_raw_buffer_load_b128(packed, (int)lane * 16, __builtin_amdgcn_readfirstlane((w_at[m] + s) * 1024), 0));
+      } else {
+        u32 at = w_at[m];
+        asm("" : "+v"(at));  // (opaque: the loads stay one uniform base and a 32-bit offset each, not a running 64-bit pointer per lane)
+        aw[m] = *(const GLOBAL v4i_any_t*)(w + s * 64 + at);
+      }
     }
   };
   // the last step's (s = last; a function of s, so that nothing of it is kept over the loop): nothing is read past the array, and the weights
@@ -156,14 +161,16 @@ __device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int p = 0; p < NP; ++p) acc[m][p] = v4i_t{0, 0, 0, 0};
-  auto multiply = [&](const v4i_t (&aw)[MT], const v4i_t* buf) {
-    const v4i_t* b = buf + wn * NP * 64 + lane;
+  auto fragments = [&](const v4i_t* buf, v4i_t (&b)[NP]) {
 #pragma unroll
-    for (int p = 0; p < NP; ++p) {
-      const v4i_t bp = b[p * 64];
+    for (int p = 0; p < NP; ++p) b[p] = buf[(wn * NP + p) * 64 + lane];
+    __builtin_amdgcn_sched_barrier(0);  // (requested together, ahead of the step's other work: one LDS latency a step)
+  };
+  auto multiply = [&](const v4i_t (&aw)[MT], const v4i_t (&b)[NP]) {
 #pragma unroll
-      for (int m = 0; m < MT; ++m) acc[m][p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(aw[m], bp, acc[m][p], 0, 0, 0);
-    }
+    for (int p = 0; p < NP; ++p)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) acc[m][p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(aw[m], b[p], acc[m][p], 0, 0, 0);
   };
   v4i_t *buf0 = frag, *buf1 = frag + WN * NP * 64;
   {
@@ -185,13 +192,16 @@ __device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a
       load_x(s + 2, raw);
     };
     for (u32 s = 0;; s += 2) {
+      v4i_t b[NP];
       lds_barrier();
+      fragments(buf0, b);
       next(s + 1, raw1, aw1, buf1);
-      multiply(aw0, buf0);
+      multiply(aw0, b);
       if (s + 1 > last) break;
       lds_barrier();
+      fragments(buf1, b);
       next(s + 2, raw0, aw0, buf0);
-      multiply(aw1, buf1);
+      multiply(aw1, b);
       if (s + 2 > last) break;
     }
   }
@@ -260,9 +270,9 @@ __device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a
   else       a.tok ? finish(F{}, T{}) : finish(F{}, F{});
 }
 
-template <int MT, int WJ, bool PACKED>
-__global__ __launch_bounds__(256, 2) void linear_i8_mfma_kernel(DevCtx c, LinearArgs a, u32 j_blocks, u32 n_blocks) {
-  __shared__ v4i_t frag[2 * (4 / WJ) * 8 * 64];
+template <int MT, int WJ, int WN, bool PACKED>
+__global__ __launch_bounds__(64 * WJ * WN, 2) void linear_i8_mfma_kernel(DevCtx c, LinearArgs a, u32 j_blocks, u32 n_blocks) {
+  __shared__ v4i_t frag[2 * WN * 8 * 64];
   // workgroups that read the same columns run side by side on one XCD (ids congruent mod 8): its L2 keeps the residues for all outputs
   const u32 cols = gridDim.x / j_blocks;
   u32 jb, cb;
@@ -280,9 +290,9 @@ __global__ __launch_bounds__(256, 2) void linear_i8_mfma_kernel(DevCtx c, Linear
   if (!owns(c, gi)) return;
   const DevPrime P = c.primes[gi];
   const u32 nb = cb % n_blocks, rc = cb / n_blocks, comp = rc % a.n_comp, row = rc / a.n_comp;
-  const u32 n0 = nb * (64 / WJ), j0 = jb * (16 * MT * WJ);
-  if (P.q <= kBytes7) linear_tile<7, MT, WJ, PACKED>(c, a, frag, P, rep, pos, row, comp, n0, j0);
-  else                linear_tile<8, MT, WJ, PACKED>(c, a, frag, P, rep, pos, row, comp, n0, j0);
+  const u32 n0 = nb * (16 * WN), j0 = jb * (16 * MT * WJ);
+  if (P.q <= kBytes7) linear_tile<7, MT, WJ, WN, PACKED>(c, a, frag, P, rep, pos, row, comp, n0, j0);
+  else                linear_tile<8, MT, WJ, WN, PACKED>(c, a, frag, P, rep, pos, row, comp, n0, j0);
 }
 
 // What the matrix-core form does not take (linear_fits: rings below 64, primes below 2^40, strides of over 32 MiB): one coefficient per lane, kJ outputs: residues split at 31 bits, so that each half times a weight is one multiply-add into a
@@ -332,18 +342,18 @@ static bool linear_fits(const DevCtx& c, const LinearArgs& a) {
          (u64)(a.n_out - 1) * a.ld_w + a.n_in >= 16;
 }
 
-template <int MT, int WJ>
+template <int MT, int WJ, int WN>
 static void launch_mfma(const DevCtx& c, const LinearArgs& a, hipStream_t s) {
-  const u32 n_blocks = c.N / (64 / WJ), j_blocks = (a.n_out + 16 * MT * WJ - 1) / (16 * MT * WJ);
+  const u32 n_blocks = c.N / (16 * WN), j_blocks = (a.n_out + 16 * MT * WJ - 1) / (16 * MT * WJ);
   const dim3 grid(n_blocks * j_blocks * a.n_comp * a.rows, a.n_limbs, c.nrep);
-  if (a.packed) hipLaunchKernelGGL((linear_i8_mfma_kernel<MT, WJ, true>), grid, dim3(256), 0, s, c, a, j_blocks, n_blocks);
-  else          hipLaunchKernelGGL((linear_i8_mfma_kernel<MT, WJ, false>), grid, dim3(256), 0, s, c, a, j_blocks, n_blocks);
+  if (a.packed) hipLaunchKernelGGL((linear_i8_mfma_kernel<MT, WJ, WN, true>), grid, dim3(64 * WJ * WN), 0, s, c, a, j_blocks, n_blocks);
+  else          hipLaunchKernelGGL((linear_i8_mfma_kernel<MT, WJ, WN, false>), grid, dim3(64 * WJ * WN), 0, s, c, a, j_blocks, n_blocks);
 }
 
 // Outputs whose packed weights fit the workspace at a time (all of them unless the layer is large); 0: the weights are read as they lie
 u32 linear_pack_outputs(const DevCtx& c, const LinearArgs& a, size_t ws_bytes) {
   if (!linear_fits(c, a) || a.n_out <= 32) return 0;
-  const u64 tile = (u64)((a.n_in + 63) / 64) * 1024, tiles = ws_bytes / tile;
+  const u64 tile = (u64)((a.n_in + 63) / 64) * 1024, tiles = std::min(ws_bytes, (size_t)1 << 31) / tile;  // (32-bit offsets)
   if (tiles * 16 >= a.n_out) return a.n_out;
   return (u32)(tiles / 16 * 256);  // whole workgroups
 }
@@ -357,15 +367,15 @@ void launch_linear_i8(const DevCtx& c, const LinearArgs& a, hipStream_t s) {
     const u32 n_blocks = (c.N + 255) / 256, j_blocks = (a.n_out + kJ - 1) / kJ;
     hipLaunchKernelGGL(linear_i8_kernel, dim3(n_blocks * j_blocks * a.n_comp * a.rows, a.n_limbs, c.nrep), dim3(256), 0, s, c, a, n_blocks, j_blocks);
   } else if (a.n_out <= 16) {
-    launch_mfma<1, 1>(c, a, s);
+    launch_mfma<1, 1, 4>(c, a, s);
   } else if (a.n_out <= 32) {
-    launch_mfma<2, 1>(c, a, s);
+    launch_mfma<2, 1, 4>(c, a, s);
   } else if (a.n_out <= 64) {
-    launch_mfma<4, 1>(c, a, s);
+    launch_mfma<4, 1, 4>(c, a, s);
   } else if (a.n_out <= 128) {
-    launch_mfma<4, 2>(c, a, s);
+    launch_mfma<4, 2, 2>(c, a, s);
   } else {
-    launch_mfma<4, 4>(c, a, s);
+    launch_mfma<4, 4, 1>(c, a, s);
   }
 }
 
