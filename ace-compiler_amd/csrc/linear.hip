@@ -76,16 +76,32 @@ __device__ __forceinline__ u64 mul_near(u64 a, u64 w, u64 wp, u64 nq) {
   return a * w + h * nq;
 }
 
+// Column blocks of a launch: 16 WN columns of one polynomial of one row.
+struct Columns {
+  u32 first, step, n;  // of a workgroup: column blocks first, first + step ..
+  u32 log_blocks;      // column blocks of a polynomial
+};
+
 template <int NP, int MT, int WJ, int WN, bool PACKED>
-__device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a, v4i_t* frag, const DevPrime& P, u32 rep, u32 pos, u32 row, u32 comp, u32 n0, u32 j0) {
-  constexpr int G = 4 / WJ;  // column blocks that a thread stages
+__device__ __forceinline__ void linear_tiles(const DevCtx& c, const LinearArgs& a, v4i_t* frag, ulong2* factor, const DevPrime& P, u32 rep, u32 pos, const Columns& cols,
+                                             u32 j0) {
+  constexpr int G = 4 / WJ;  // column blocks of 16 that a thread stages
   const u32 t = threadIdx.x, lane = t & 63u, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const u32 wj = wave % WJ, wn = wave / WJ;
-  const u64 off = (u64)pos * c.N + n0;
   const u32 last = (a.n_in - 1) / 64;  // step (n_in > 0)
+  const u64 q = P.q, mh = P.prec128_hi;
+  // where a column block starts in a matrix (uniform)
+  auto block = [&](u32 i, const CtMat& m, u64* base, u32& row, u64& off) {
+    const u32 cb = cols.first + i * cols.step, rc = cb >> cols.log_blocks;
+    row = __builtin_amdgcn_readfirstlane(rc / a.n_comp);
+    const u32 comp = rc - row * a.n_comp;
+    off = (u64)pos * c.N + (cb & ((1u << cols.log_blocks) - 1)) * (16 * WN);
+    return uniform(base + row * m.row + comp * m.comp + off);
+  };
+  u64* const x_base = reb(c, a.in.d, rep);
+  u64* const y_base = reb(c, a.out.d, rep);
   // addresses: a uniform 64-bit base that moves with the step plus 32-bit offsets of the lanes that stay (linear_fits)
   const u64 xs = a.in.col;
-  const u64* x = uniform(reb(c, a.in.d, rep) + row * a.in.row + comp * a.in.comp + off);
   const u32 k4 = (t >> 4) & 15u, u0 = t >> 8;  // this thread stages inputs 4 k4 .. 4 k4 + 3 of a step in column blocks u0, u0 + WN / G ..
   u32 x_at[4];
 #pragma unroll
@@ -100,14 +116,26 @@ __device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a
   struct Raw {
     u64 v[G][4];
   };
-  // a step's inputs through a buffer descriptor that ends behind the last of them: those past n_in read as zero
-  auto load_x = [&](u32 s, Raw& r) {
-    const int there = max(min((int)a.n_in - (int)s * 64, 64), 0);
-    const auto d = __builtin_amdgcn_make_buffer_rsrc((void*)uniform(x + (u64)s * 64 * xs), 0, __builtin_amdgcn_readfirstlane(there * (int)xs * 8), 0x00027000);
+  // the inputs of (tile, step) in their order, through a buffer descriptor that ends behind the last of them: those past n_in read as zero, and
+  // behind the last tile nothing is read.  No branch (the steps are one block of code): x_next is made ready once a tile.
+  u32 x_tile = 0, x_step = 0, any_row;
+  u64 any_off;
+  int x_rest = (int)a.n_in;
+  const int limb64 = (int)xs * 512;  // bytes of a whole step
+  const u64* x = block(0, a.in, x_base, any_row, any_off);
+  const u64* x_next = block(1, a.in, x_base, any_row, any_off);
+  auto load_x = [&](Raw& r) {
+    const int bytes = x_rest >= 64 ? limb64 : x_rest > 0 ? x_rest * (int)xs * 8 : 0;
+    const auto d = __builtin_amdgcn_make_buffer_rsrc((void*)x, 0, bytes, 0x00027000);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int u = 0; u < G; ++u) r.v[u][i] = __builtin_bit_cast(u64, __builtin_amdgcn_raw_buffer_load_b64(d, (int)x_at[i] + u * (WN / G * 128), 0, 0));
+    const bool wrap = x_step == (last | 1u);
+    x_step = wrap ? 0 : x_step + 1;
+    x_tile += wrap;
+    x_rest = wrap ? (x_tile < cols.n ? (int)a.n_in : 0) : x_rest - 64;
+    x = wrap ? x_next : x + 64 * xs;
   };
   auto stage = [&](const Raw& r, v4i_t* buf) {
     constexpr u64 C = NP == 8 ? 0x8080808080808080ull : 0x80808080808080ull;
@@ -157,81 +185,59 @@ __device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a
   };
 
   v4i_t acc[MT][NP];
+  auto clear = [&] {
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int p = 0; p < NP; ++p) acc[m][p] = v4i_t{0, 0, 0, 0};
-  auto fragments = [&](const v4i_t* buf, v4i_t (&b)[NP]) {
-#pragma unroll
-    for (int p = 0; p < NP; ++p) b[p] = buf[(wn * NP + p) * 64 + lane];
-    __builtin_amdgcn_sched_barrier(0);  // (requested together, ahead of the step's other work: one LDS latency a step)
+      for (int p = 0; p < NP; ++p) acc[m][p] = v4i_t{0, 0, 0, 0};
   };
-  auto multiply = [&](const v4i_t (&aw)[MT], const v4i_t (&b)[NP]) {
+  // the B fragments of a step four planes ahead of their use: one LDS latency a step, 16 registers
+  constexpr int AHEAD = 4;
+  auto fragments = [&](const v4i_t* buf, v4i_t (&b)[AHEAD]) {
 #pragma unroll
-    for (int p = 0; p < NP; ++p)
-#pragma unroll
-      for (int m = 0; m < MT; ++m) acc[m][p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(aw[m], b[p], acc[m][p], 0, 0, 0);
+    for (int p = 0; p < AHEAD; ++p) b[p] = buf[(wn * NP + p) * 64 + lane];
+    __builtin_amdgcn_sched_barrier(0);
   };
-  v4i_t *buf0 = frag, *buf1 = frag + WN * NP * 64;
-  {
-    Raw raw0, raw1;
-    v4i_t aw0[MT], aw1[MT];
-    load_x(0, raw0);
-    load_x(1, raw1);
-    if (last == 0) load_w_last(0, aw0);
-    else           load_w(0, aw0);
-    stage(raw0, buf0);
-    load_x(2, raw0);
-    // a step: the next one's fragments are staged while this one's are multiplied.  Past the last step weights are read again and inputs as
-    // zeros, never to be used: without a branch around the requests the compiler counts them exactly and waits for the oldest only
-    auto next = [&](u32 s, Raw& raw, v4i_t (&aw)[MT], v4i_t* buf) {
-      if (!PACKED && s >= last) load_w_last(last, aw);
-      else                      load_w(min(s, last), aw);
-      __builtin_amdgcn_sched_barrier(0);  // (weights first: the next step waits for them and not for the inputs behind them)
-      stage(raw, buf);
-      load_x(s + 2, raw);
-    };
-    for (u32 s = 0;; s += 2) {
-      v4i_t b[NP];
-      lds_barrier();
-      fragments(buf0, b);
-      next(s + 1, raw1, aw1, buf1);
-      multiply(aw0, b);
-      if (s + 1 > last) break;
-      lds_barrier();
-      fragments(buf1, b);
-      next(s + 2, raw0, aw0, buf0);
-      multiply(aw1, b);
-      if (s + 2 > last) break;
+  auto multiply = [&](const v4i_t (&aw)[MT], const v4i_t* buf, v4i_t (&b)[AHEAD]) {
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) acc[m][p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(aw[m], b[p % AHEAD], acc[m][p], 0, 0, 0);
+      if (p + AHEAD < NP) b[p % AHEAD] = buf[(wn * NP + p + AHEAD) * 64 + lane];
+      __builtin_amdgcn_sched_barrier(0x36);  // (arithmetic and requests to memory may cross, LDS reads and matrix instructions not)
     }
-  }
+  };
 
-  // lane: column lane % 16, outputs 4 (lane / 16) + r of each tile.  V = sum_p acc_p 256^p is reduced by its rounded quotient in floating point:
-  // |V / q| <= 2^7 n_in <= 2^23, and what the doubles leave out of V (its low 32 bits, roundings of two units of 2^32) is below 2^-6 q at primes
-  // above 2^40.  V - round(V / q) q is then within (1/2 + 2^-5) q of zero, so its low 64 bits tell it.
-  const u64 q = P.q, mh = P.prec128_hi;
-  const u32 n = wn * 16 + (lane & 15u), g4 = 4 * (lane >> 4);
-  GLOBAL char* y = (GLOBAL char*)global(uniform(reb(c, a.out.d, rep) + row * a.out.row + comp * a.out.comp + off + (u64)(j0 + wj * MT * 16) * a.out.col));
+  // ---- a tile's results.  Lane: column lane % 16, outputs 4 (lane / 16) + r of each tile.  V = sum_p acc_p 256^p is reduced by its rounded quotient in
+  // floating point: |V / q| <= 2^7 n_in <= 2^23, and what the doubles leave out of V (its low 32 bits, roundings of two units of 2^32) is below
+  // 2^-6 q at primes above 2^40.  V - round(V / q) q is then within (1/2 + 2^-5) q of zero, so its low 64 bits tell it.
+  const u32 g4 = 4 * (lane >> 4), n = wn * 16 + (lane & 15u);
   const u32 y_at = 8 * (g4 * (u32)a.out.col + n);
   const u32 left = a.n_out - j0 - min(a.n_out - j0, wj * MT * 16);  // outputs of this wave that are there
-  const u64 tok = a.tok ? global(reb(c, a.tok, rep))[row * a.tok_stride + off + n] : 0;
-  const u64 tokp = tok * mh + mulhi64(tok, P.prec128_lo), nq = 0 - q;
-  const double inv = 4294967296.0 / (double)q;
-  double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the rounded integer, plus those of the constant
-  u64 start = __builtin_bit_cast(u64, magic) * q;
-  asm volatile("" : "+s"(magic), "+s"(start));
-  int weight[4] = {1, 1 << 8, 1 << 16, 1 << 24};
-  asm volatile("" : "+s"(weight[0]), "+s"(weight[1]), "+s"(weight[2]), "+s"(weight[3]));  // opaque: each byte's sum joins by ONE v_mad_i64_i32
-  ulong2* factor = (ulong2*)frag;  // channel factors and their companions
-  if (a.mul) {
-    lds_barrier();
-    if (t < 16 * MT * WJ) {
-      const u64 m = signed_mod(global(reb(c, a.mul, rep))[min(j0 + t, a.n_out - 1)], q, mh);
-      factor[t] = ulong2{m, m * mh + mulhi64(m, P.prec128_lo)};
-    }
-    lds_barrier();
+  const u64 nq = 0 - q;
+  const double inv = __builtin_bit_cast(double, (u64)uniform((char*)__builtin_bit_cast(u64, 4294967296.0 / (double)q)));
+  if (a.mul && t < 16 * MT * WJ) {  // channel factors and their companions (read behind the first barrier of the steps)
+    const u64 m = signed_mod(global(reb(c, a.mul, rep))[min(j0 + t, a.n_out - 1)], q, mh);
+    factor[t] = ulong2{m, m * mh + mulhi64(m, P.prec128_lo)};
   }
+  u32 tile = 0, row;
+  u64 off, tok = 0;
+  GLOBAL char* y;
+  auto begin = [&] {
+    x_next = block(x_tile + 1, a.in, x_base, any_row, any_off);
+    y = (GLOBAL char*)global(block(tile, a.out, y_base, row, off) + (u64)(j0 + wj * MT * 16) * a.out.col);
+    y = (GLOBAL char*)uniform((char*)y);
+    if (a.tok) tok = global(uniform(reb(c, a.tok, rep) + row * a.tok_stride + off))[n];
+    clear();
+  };
   auto finish = [&](auto with_mul, auto with_tok) {
+    const u64 tokp = tok * mh + mulhi64(tok, P.prec128_lo);
+    double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the rounded integer, plus those of the constant
+    u64 start = __builtin_bit_cast(u64, magic) * q, col = a.out.col * 8;
+    int weight[4] = {1, 1 << 8, 1 << 16, 1 << 24};
+    // (opaque: each byte's sum joins by ONE v_mad_i64_i32, and nothing made of these is kept over the steps)
+    asm volatile("" : "+s"(magic), "+s"(start), "+s"(col), "+s"(weight[0]), "+s"(weight[1]), "+s"(weight[2]), "+s"(weight[3]));
+    GLOBAL char* at = y;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -261,38 +267,77 @@ __device__ __forceinline__ void linear_tile(const DevCtx& c, const LinearArgs& a
         } else {
           v += q & (u64)((int64_t)v >> 63);
         }
-        if (m * 16 + r + g4 < left) *(GLOBAL u64*)(y + (u64)(m * 16 + r) * a.out.col * 8 + y_at) = v;
+        if (m * 16 + r + g4 < left) *(GLOBAL u64*)(at + y_at) = v;
+        at += r == 3 ? 13 * col : col;
       }
   };
-  using T = std::true_type;
-  using F = std::false_type;
-  if (a.mul) a.tok ? finish(T{}, T{}) : finish(T{}, F{});
-  else       a.tok ? finish(F{}, T{}) : finish(F{}, F{});
+  auto store = [&] {
+    using T = std::true_type;
+    using F = std::false_type;
+    if (a.mul) a.tok ? finish(T{}, T{}) : finish(T{}, F{});
+    else       a.tok ? finish(F{}, T{}) : finish(F{}, F{});
+  };
+
+  // ---- the steps of all tiles in one pipeline: inputs are requested three steps ahead and staged one ahead, across the tiles' borders, so that
+  // a tile's first inputs are under way while the one before it is reduced.  Steps go in pairs (the second of the last pair may be empty).  Behind
+  // the last step weights are read again and inputs as zeros, never to be used: without a branch around the requests the compiler counts them
+  // exactly and waits for the oldest only.
+  v4i_t *buf0 = frag, *buf1 = frag + WN * NP * 64;
+  Raw raw0, raw1;
+  v4i_t aw0[MT], aw1[MT];
+  load_x(raw0);
+  load_x(raw1);
+  if (!PACKED && last == 0) load_w_last(0, aw0);
+  else                      load_w(0, aw0);
+  stage(raw0, buf0);
+  load_x(raw0);
+  auto step = [&](u32 ahead, bool full, const v4i_t* buf, const v4i_t (&aw)[MT], Raw& raw, v4i_t* buf_next, v4i_t (&aw_next)[MT]) {
+    v4i_t b[AHEAD];
+    lds_barrier();
+    fragments(buf, b);
+    if (!PACKED && ahead == last) load_w_last(ahead, aw_next);
+    else                          load_w(ahead, aw_next);
+    __builtin_amdgcn_sched_barrier(0);  // (weights first: the next step waits for them and not for the inputs behind them)
+    stage(raw, buf_next);
+    load_x(raw);
+    if (full) multiply(aw, buf, b);
+  };
+  for (tile = 0; tile < cols.n; ++tile) {
+    begin();
+    for (u32 s = 0; s <= last; s += 2) {
+      step(min(s + 1, last), true, buf0, aw0, raw1, buf1, aw1);
+      step(s + 2 > last ? 0 : s + 2, s + 1 <= last, buf1, aw1, raw0, buf0, aw0);
+    }
+    store();
+  }
 }
 
+// A workgroup takes `tiles` column blocks one after the other; the rest of them go by launch_mfma's order.
 template <int MT, int WJ, int WN, bool PACKED>
-__global__ __launch_bounds__(64 * WJ * WN, 2) void linear_i8_mfma_kernel(DevCtx c, LinearArgs a, u32 j_blocks, u32 n_blocks) {
+__global__ __launch_bounds__(64 * WJ * WN, 2) void linear_i8_mfma_kernel(DevCtx c, LinearArgs a, u32 j_blocks, u32 log_blocks, u32 tiles) {
   __shared__ v4i_t frag[2 * WN * 8 * 64];
+  __shared__ ulong2 factor[16 * MT * WJ];
   // workgroups that read the same columns run side by side on one XCD (ids congruent mod 8): its L2 keeps the residues for all outputs
-  const u32 cols = gridDim.x / j_blocks;
-  u32 jb, cb;
-  if ((cols & 7u) == 0) {
+  const u32 groups = gridDim.x / j_blocks;
+  u32 jb, g;
+  if ((groups & 7u) == 0) {
     const u32 b = blockIdx.x >> 3;
     jb = b % j_blocks;
-    cb = (b / j_blocks) * 8 + (blockIdx.x & 7u);
+    g = (b / j_blocks) * 8 + (blockIdx.x & 7u);
   } else {
     jb = blockIdx.x % j_blocks;
-    cb = blockIdx.x / j_blocks;
+    g = blockIdx.x / j_blocks;
   }
   jb = __builtin_amdgcn_readfirstlane(jb);
-  cb = __builtin_amdgcn_readfirstlane(cb);
+  g = __builtin_amdgcn_readfirstlane(g);
   const u32 pos = a.pos0 + blockIdx.y, gi = limb_prime(pos, a.level, c.L), rep = c.rep0 + blockIdx.z;
   if (!owns(c, gi)) return;
   const DevPrime P = c.primes[gi];
-  const u32 nb = cb % n_blocks, rc = cb / n_blocks, comp = rc % a.n_comp, row = rc / a.n_comp;
-  const u32 n0 = nb * (16 * WN), j0 = jb * (16 * MT * WJ);
-  if (P.q <= kBytes7) linear_tile<7, MT, WJ, WN, PACKED>(c, a, frag, P, rep, pos, row, comp, n0, j0);
-  else                linear_tile<8, MT, WJ, WN, PACKED>(c, a, frag, P, rep, pos, row, comp, n0, j0);
+  const u32 all = (a.rows * a.n_comp) << log_blocks;
+  const Columns cols{g * tiles, 1, min(tiles, all - g * tiles), log_blocks};
+  const u32 j0 = jb * (16 * MT * WJ);
+  if (P.q <= kBytes7) linear_tiles<7, MT, WJ, WN, PACKED>(c, a, frag, factor, P, rep, pos, cols, j0);
+  else                linear_tiles<8, MT, WJ, WN, PACKED>(c, a, frag, factor, P, rep, pos, cols, j0);
 }
 
 // What the matrix-core form does not take (linear_fits: rings below 64, primes below 2^40, strides of over 32 MiB): one coefficient per lane, kJ outputs: residues split at 31 bits, so that each half times a weight is one multiply-add into a
@@ -344,10 +389,16 @@ static bool linear_fits(const DevCtx& c, const LinearArgs& a) {
 
 template <int MT, int WJ, int WN>
 static void launch_mfma(const DevCtx& c, const LinearArgs& a, hipStream_t s) {
-  const u32 n_blocks = c.N / (16 * WN), j_blocks = (a.n_out + 16 * MT * WJ - 1) / (16 * MT * WJ);
-  const dim3 grid(n_blocks * j_blocks * a.n_comp * a.rows, a.n_limbs, c.nrep);
-  if (a.packed) hipLaunchKernelGGL((linear_i8_mfma_kernel<MT, WJ, WN, true>), grid, dim3(64 * WJ * WN), 0, s, c, a, j_blocks, n_blocks);
-  else          hipLaunchKernelGGL((linear_i8_mfma_kernel<MT, WJ, WN, false>), grid, dim3(64 * WJ * WN), 0, s, c, a, j_blocks, n_blocks);
+  u32 log_blocks = 0;
+  while ((16u * WN << log_blocks) < c.N) ++log_blocks;
+  const u32 all = (a.rows * a.n_comp) << log_blocks, j_blocks = (a.n_out + 16 * MT * WJ - 1) / (16 * MT * WJ);
+  // several column blocks to a workgroup once the card is filled a few times over (two workgroups on each of 256 CUs)
+  const u64 blocks = (u64)all * j_blocks * a.n_limbs * c.nrep;
+  u32 tiles = 1;
+  while (tiles < 8 && blocks / (2 * tiles) >= 2048) tiles *= 2;
+  const dim3 grid((all + tiles - 1) / tiles * j_blocks, a.n_limbs, c.nrep), block(64 * WJ * WN);
+  if (a.packed) hipLaunchKernelGGL((linear_i8_mfma_kernel<MT, WJ, WN, true>), grid, block, 0, s, c, a, j_blocks, log_blocks, tiles);
+  else          hipLaunchKernelGGL((linear_i8_mfma_kernel<MT, WJ, WN, false>), grid, block, 0, s, c, a, j_blocks, log_blocks, tiles);
 }
 
 // Outputs whose packed weights fit the workspace at a time (all of them unless the layer is large); 0: the weights are read as they lie

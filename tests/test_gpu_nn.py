@@ -185,6 +185,46 @@ def test_linear_longest_sum(contexts):
     x.free()
 
 
+def mul_mod(a, b, q):
+    """a * b mod q for uint64 a, b < q < 2^61: quotient from a product in 64 bits of mantissa, at most one off"""
+    f = np.floor(a.astype(np.longdouble) * b.astype(np.longdouble) / q.astype(np.longdouble)).astype(np.uint64)
+    r = (a * b - f * q).astype(np.int64)
+    q = q.astype(np.int64)
+    r = np.where(r < 0, r + q, r)
+    return np.where(r >= q, r - q, r).astype(np.uint64)
+
+
+@pytest.mark.parametrize("n_in,n_out,rows,n_comp", [(65, 257, 1, 2), (40, 300, 1, 2), (129, 144, 3, 1), (192, 260, 1, 3), (3, 33, 5, 3)])
+def test_linear_many_column_blocks(contexts, n_in, n_out, rows, n_comp):
+    """large enough a ring that a workgroup takes several column blocks, across polynomials and rows"""
+    rt = _open.setdefault("n16384", A.AceHip(16384, 2, 60, 50, 1))
+    level, limbs, N = 2, [0, 1, 2], rt.N
+    q = np.array([rt.primes[i] for i in range(3)], dtype=np.uint64)[:, None]
+    rng = np.random.default_rng(n_in)
+    x = np.stack([rng.integers(0, p[0], size=(rows, n_in, n_comp, N), dtype=np.uint64) for p in q], axis=-2)   # [row][i][comp][limb][N]
+    w, m = rng.integers(-128, 128, size=(n_out, n_in)).astype(np.int8), rng.integers(-(1 << 62), 1 << 62, size=n_out)
+    tok = np.stack([rng.integers(0, p[0], size=(rows, N), dtype=np.uint64) for p in q], axis=-2)
+    dx, dw, dm, dt, dy = dev(rt, x), dev(rt, w), dev(rt, m), dev(rt, tok), dev(rt, np.full((rows, n_out, n_comp, 3, N), 7, np.uint64))
+    strides = lambda n: dict(row=n * n_comp * 3 * N, col=n_comp * 3 * N, comp=3 * N)
+    rt.linear_i8(rt.mat(dy.ptr, **strides(n_out)), rt.mat(dx.ptr, **strides(n_in)), dw.ptr, n_in, rows, n_in, n_out, n_comp, level, n_limbs=3, d_mul=dm.ptr, d_tok=dt.ptr,
+                 tok_stride=3 * N)
+    some = np.unique(np.concatenate([[0, n_out - 1], rng.integers(0, n_out, size=14)]))   # outputs that are compared
+    got = dy.download((rows, n_out, n_comp, 3, N))[:, some]
+    w, m, n_out = w[some], m[some], len(some)
+    flat = x.transpose(1, 0, 2, 3, 4).reshape(n_in, -1)
+    parts = [(w.astype(np.float64) @ (flat >> np.uint64(s) & np.uint64((1 << 20) - 1)).astype(np.float64)).astype(np.int64) for s in (0, 20, 40)]   # exact: below 2^38
+    parts = [p.reshape(n_out, rows, n_comp, 3, N) for p in parts]
+    qi = q.astype(np.int64)
+    y = np.zeros_like(parts[0], dtype=np.uint64)
+    for p in parts[::-1]:
+        y = ((mul_mod(y, np.broadcast_to(np.uint64(1 << 20), y.shape), q) + (p % qi).astype(np.uint64)) % q).astype(np.uint64)
+    factor = np.array([[int(a) % int(b) for b in q[:, 0]] for a in m], dtype=np.uint64)
+    y = mul_mod(mul_mod(y, np.broadcast_to(factor[:, None, None, :, None], y.shape), q), np.broadcast_to(tok[None, :, None], y.shape), q)
+    assert np.array_equal(got, y.transpose(1, 0, 2, 3, 4))
+    for d in (dx, dw, dm, dt, dy):
+        d.free()
+
+
 def test_linear_empty_sum_is_zero(contexts):
     linear_case(contexts("n64"), 2, [0, 1], 1, 0, 5, 2, True, True)
 
