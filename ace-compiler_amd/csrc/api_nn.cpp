@@ -30,6 +30,11 @@ struct Call {
     if (pos0 > level + c->hp.K || n_limbs > level + c->hp.K - pos0) return bad("limb range exceeds level + K");
     return ACEHIP_OK;
   }
+  bool primes_above(u32 bits) const {
+    for (u32 p = pos0; p < pos0 + n_limbs; ++p)
+      if (c->hp.q(limb_prime(p, level, c->hp.L)) >> bits == 0) return false;
+    return true;
+  }
   int view(View& v, const acehip_mat* a, u64 heads, u64 rows, u64 cols, u64 comps) const {
     v.n[0] = heads, v.n[1] = rows, v.n[2] = cols, v.n[3] = comps;
     v.limb0 = 8ull * pos0 * c->hp.N;
@@ -160,8 +165,7 @@ int acehip_linear_i8(acehip_ctx* c, const acehip_mat* out, const acehip_mat* in,
   a.tok_stride = tok_stride;
   a.rows = rows, a.n_in = n_in, a.n_out = n_out, a.n_comp = n_comp;
   a.level = level, a.pos0 = pos0, a.n_limbs = n_limbs;
-  a.wide_primes = true;
-  for (u32 p = pos0; p < pos0 + n_limbs; ++p) a.wide_primes = a.wide_primes && c->hp.q(limb_prime(p, level, c->hp.L)) >> 40;
+  a.wide_primes = k.primes_above(40);
   // (weights inside the arena differ from replica to replica: they are read as they lie)
   const bool shared = c->dc.rep_span == 0 || (u64)(uintptr_t)d_w - c->dc.rep_lo >= c->dc.rep_span;
   const u32 part = shared ? linear_pack_outputs(c->dc, a, c->ws_words * sizeof(u64)) : 0;
@@ -261,10 +265,11 @@ static u64 seen(u64 n_q, u64 n_k, int causal) {
 }
 static int run_linattn(const Call& k, LinattnArgs& a, const View& y, u64 polys, acehip_stream s) {
   acehip_ctx* c = k.c;
-  if (int e = check_blocks(k, (i128)((c->hp.N + 255) / 256) * a.Nn * a.M * a.n_heads)) return e;
+  if (int e = check_blocks(k, (i128)((c->hp.N + 63) / 64) * a.Nn * a.M * a.n_heads)) return e;
   if (int e = check_dev(c)) return e;
   a.out = y.m;
   a.level = k.level, a.pos0 = k.pos0, a.n_limbs = k.n_limbs;
+  a.wide_primes = k.primes_above(32);
   for (const DevCtx& dc : launch_dcs(c)) launch_linattn(dc, a, (hipStream_t)s);
   stat(ST_LINATTN, (u64)a.n_heads * a.M * a.Nn, polys * 8ull * c->hp.N * k.n_limbs);
   return post_launch();

@@ -7,7 +7,7 @@ namespace acehip {
 //   x*y = ll + ((xl + xh)(yl + yh) - ll - hh) 2^hb + hh 2^(2 hb)
 // take one 32x32 multiply-add each.  mm may wrap on the way: only the difference mm - ll - hh counts.  For primes of n bits a product's
 // middle part is below 2^(n+1), and an accumulator takes at most two products a term, so 2^(62-n) terms stay below 2^64 (the exact bound
-// 2^(64-n) (2^hb - 1)(2^(n-hb) - 1) leaves room for the residue that the sums start from); then the sums are brought back to one residue.
+// 2^(64-n) (2^hb - 1)(2^(n-hb) - 1) leaves room for what carry() leaves in the sums); then carry() makes room again.
 struct Half {
   u32 l, h, s;
 };
@@ -16,102 +16,227 @@ __device__ __forceinline__ Half halves(u64 x, u32 hb) {
   return Half{l, h, l + h};
 }
 struct Acc {
-  u64 ll = 0, mm = 0, hh = 0;
+  u64 ll, mm, hh;
   __device__ __forceinline__ void mac(const Half& x, const Half& y) {
     ll += (u64)x.l * y.l;
     mm += (u64)x.s * y.s;
     hh += (u64)x.h * y.h;
   }
+  template <bool WIDE>
   __device__ __forceinline__ u64 value(u32 hb, const DevPrime& P) const {
     unsigned __int128 v = ll;
     v += (unsigned __int128)(mm - ll - hh) << hb;
     v += (unsigned __int128)hh << (2 * hb);
-    return reduce128(U128{(u64)v, (u64)(v >> 64)}, P.q, P.prec128_lo, P.prec128_hi);
+    const U128 x{(u64)v, (u64)(v >> 64)};
+    return WIDE ? reduce128(x, P.q, P.prec128_lo, (u32)P.prec128_hi) : reduce128_generic(x, P.q, P.prec128_lo, P.prec128_hi);
   }
-  __device__ __forceinline__ void fold(u32 hb, const DevPrime& P) {
-    const Half v = halves(value(hb, P), hb);
-    ll = v.l;
-    hh = 0;
-    mm = (u64)v.l + v.h;
+  // carries brought up and hh reduced below 2q: room for as many terms again
+  __device__ __forceinline__ void carry(u32 hb, u64 q, u64 mh) {
+    const u64 mask = (1ull << hb) - 1;
+    u64 mid = mm - ll - hh + (ll >> hb);
+    ll &= mask;
+    hh += mid >> hb;
+    mid &= mask;
+    hh -= mulhi64(hh, mh) * q;
+    mm = mid + ll + hh;
   }
 };
 
-__global__ __launch_bounds__(256) void linattn_kernel(DevCtx c, LinattnArgs a, u32 n_blocks) {
+#define GLOBAL __attribute__((address_space(1)))
+// a pointer that is the same for the wave, on the scalar unit (lanes add their coefficient as a 32-bit offset)
+__device__ __forceinline__ const GLOBAL char* uniform(const u64* p) {
+  const u64 v = (u64)p;
+  return (const GLOBAL char*)(((u64)(u32)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) | (u32)__builtin_amdgcn_readfirstlane((int)v));
+}
+
+// A wave: 64 coefficients, MT x NT results (3 sums of 3 words each); a workgroup: WM x WN such tiles of the same coefficients, whose operands
+// meet in the CU's L1.  Per term of the sums a lane reads 2 (MT + NT) residues and makes 12 MT NT multiply-adds.
+// WIDE: primes above 2^32 (the reduction's quotient from three partial products).
+template <int MT, int NT, int WM, int WN, bool WIDE>
+__global__ __launch_bounds__(64 * WM * WN, 2) void linattn_kernel(DevCtx c, LinattnArgs a, u32 n_blocks, u32 m_tiles, u32 n_tiles) {
+  constexpr u32 KC = 64;  // terms whose factors are prepared at a time
+  __shared__ ulong2 factor[KC + MT * WM];
   u32 b = blockIdx.x;
-  const u32 nb = b % n_blocks;
-  b /= n_blocks;
-  const u32 j = b % a.Nn;
-  b /= a.Nn;
-  const u32 m = b % a.M, h = b / a.M, rep = c.rep0 + blockIdx.z;
+  // tiles of the same coefficients follow each other on one XCD (ids congruent mod 8): its L2 keeps their operands
+  const u32 groups = gridDim.x / (m_tiles * n_tiles);
+  u32 g, t;
+  if ((groups & 7u) == 0) {
+    const u32 x = b >> 3;
+    t = x % (m_tiles * n_tiles);
+    g = (x / (m_tiles * n_tiles)) * 8 + (b & 7u);
+  } else {
+    t = b % (m_tiles * n_tiles);
+    g = b / (m_tiles * n_tiles);
+  }
+  t = __builtin_amdgcn_readfirstlane(t);
+  g = __builtin_amdgcn_readfirstlane(g);
+  const u32 nb = g % n_blocks, h = g / n_blocks, rep = c.rep0 + blockIdx.z;
+  const u32 lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const u32 wg_m = (t / n_tiles) * (MT * WM), m0 = wg_m + (wave / WN) * MT, j0 = ((t % n_tiles) * WN + wave % WN) * NT;
   const u32 pos = a.pos0 + blockIdx.y, gi = limb_prime(pos, a.level, c.L);
-  const u32 n = nb * 256 + threadIdx.x;
-  if (!owns(c, gi) || n >= c.N) return;
-  const int64_t last = (int64_t)m + a.off;  // last column / key that row m sees
-  if (a.skip_above && (int64_t)j > last) return;
+  if (!owns(c, gi)) return;
+  const int64_t off = a.off;
+  // last column / key that the rows of the workgroup and of this wave see (rows past M: the last one's)
+  const int64_t wg_last = (int64_t)min(wg_m + MT * WM, a.M) - 1 + off, last = (int64_t)min(m0 + MT, a.M) - 1 + off;
+  if (a.skip_above && (int64_t)((t % n_tiles) * (NT * WN)) > wg_last) return;
   const DevPrime P = c.primes[gi];
   const u64 q = P.q, mh = P.prec128_hi;
   const u32 hb = (P.nbits + 1) / 2;
+  const u32 n = nb * 64 + lane, at = 8 * min(n, c.N - 1);  // (rings below 64: the lanes behind the ring repeat its last coefficient and store nothing)
+  const u64 limb = (u64)pos * c.N;
+  u32 row[MT], col[NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) row[i] = min(m0 + i, a.M - 1);
+#pragma unroll
+  for (int i = 0; i < NT; ++i) col[i] = min(j0 + i, a.Nn - 1);
+  auto read = [&](const u64* p) { return *(const GLOBAL u64*)(uniform(p) + at); };
+
+  Acc s[MT][NT][3];
   const u32 period = 1u << min(62 - P.nbits, 24u);
-  const u64 off = (u64)pos * c.N + n;
-  u64 r[3] = {0, 0, 0};
-  auto term = [&](const LinattnTerm& t, u32 K, bool weighted) {
-    const u64* A = reb(c, t.a.d, rep) + (h / t.a_group) * t.a.head + m * t.a.row + off;
-    const u64* B = reb(c, t.b.d, rep) + (h / t.b_group) * t.b.head + j * t.b.col + off;
-    const int64_t* w = weighted ? reb(c, a.decay, rep) + h * a.decay_ld : nullptr;
-    Acc s0, s1, s2;
-    u32 left = period;
-    for (u32 k = 0; k < K; ++k) {
-      u64 a0 = A[k * t.a.col], a1 = A[k * t.a.col + t.a.comp];
-      const Half b0 = halves(B[k * t.b.row], hb), b1 = halves(B[k * t.b.row + t.b.comp], hb);
-      if (w) {
-        const u64 d = signed_mod(w[a.decay_by_k ? (u64)(t.K - 1 - k) : (u64)(last - k)], q, mh);
-        a0 = mul_mod(a0, d, P);
-        a1 = mul_mod(a1, d, P);
-      }
-      const Half h0 = halves(a0, hb), h1 = halves(a1, hb);
-      if (left == 0) {
-        s0.fold(hb, P);
-        s1.fold(hb, P);
-        s2.fold(hb, P);
-        left = period;
-      }
-      --left;
-      s0.mac(h0, b0);
-      s1.mac(h0, b1);
-      s1.mac(h1, b0);
-      s2.mac(h1, b1);
-    }
-    return ulong3{s0.value(hb, P), s1.value(hb, P), s2.value(hb, P)};
+  u32 left = period;  // terms that the sums still take
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int p = 0; p < 3; ++p) s[i][j][p] = Acc{0, 0, 0};
+  if (a.base.d) {  // one term: keep * base
+    const u64* S = reb(c, a.base.d, rep) + h * a.base.head + limb;
+    const Half f = halves(a.keep ? signed_mod(reb(c, a.keep, rep)[h], q, mh) : 1, hb);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) s[i][j][p].mac(halves(read(S + row[i] * a.base.row + col[j] * a.base.col + p * a.base.comp), hb), f);
+    --left;
+  }
+  struct Raw {
+    u64 a[MT][2], b[NT][2];
   };
-  if (a.t1.K) {
-    const ulong3 v = term(a.t1, a.t1.K, false);
-    r[0] = v.x;
-    r[1] = v.y;
-    r[2] = v.z;
-    if (a.scale) {
-      const u64 g = signed_mod(reb(c, a.scale, rep)[h * a.M + m], q, mh);
-      for (int p = 0; p < 3; ++p) r[p] = mul_mod(r[p], g, P);
+#pragma unroll 1
+  for (u32 part = 0; part < 2; ++part) {
+    const LinattnTerm& t = part ? a.t2 : a.t1;
+    const bool causal = part && a.causal, weighted = part ? a.decay != nullptr : a.scale != nullptr;
+    // a causal sum ends with the last key that a row of the wave (of the workgroup: the factors) sees
+    const u32 K = causal ? (u32)min((int64_t)t.K, max(last + 1, (int64_t)0)) : t.K, K_wg = causal ? (u32)min((int64_t)t.K, max(wg_last + 1, (int64_t)0)) : t.K;
+    if (K_wg == 0) continue;
+    const u64* A = reb(c, t.a.d, rep) + (h / t.a_group) * t.a.head + limb;
+    const u64* B = reb(c, t.b.d, rep) + (h / t.b_group) * t.b.head + limb;
+    const u64 a_col = t.a.col, b_row = t.b.row;
+    const u64 *pa[MT][2], *pb[NT][2];  // where the next term's residues lie
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) pa[i][p] = A + row[i] * t.a.row + p * t.a.comp;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) pb[i][p] = B + col[i] * t.b.col + p * t.b.comp;
+    auto load = [&](Raw& r, bool more) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          r.a[i][p] = read(pa[i][p]);
+          pa[i][p] += more ? a_col : 0;
+        }
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          r.b[i][p] = read(pb[i][p]);
+          pb[i][p] += more ? b_row : 0;
+        }
+    };
+    Raw next;
+    load(next, K > 1);
+    for (u32 k0 = 0; k0 < K_wg; k0 += KC) {
+      if (weighted) {
+        // factors of the terms from k0 on: term 1's by row; term 2's by term, or by distance (entry e: the distance that row wg_m meets at term
+        // k0 + KC - 1, and so on upwards)
+        __syncthreads();
+        for (u32 e = threadIdx.x; e < KC + MT * WM; e += 64 * WM * WN) {
+          const int64_t d = part == 0 ? (int64_t)min(wg_m + e, a.M - 1) : a.decay_by_k ? (int64_t)t.K - 1 - k0 - e : (int64_t)wg_m + off - (k0 + KC - 1) + e;
+          const bool there = d >= 0 && d < (int64_t)(part ? t.K : a.M);
+          const u64 f = there ? signed_mod(part ? reb(c, a.decay, rep)[h * a.decay_ld + d] : reb(c, a.scale, rep)[h * a.M + d], q, mh) : 0;
+          factor[e] = ulong2{f, f * mh + mulhi64(f, P.prec128_lo)};
+        }
+        __syncthreads();
+      }
+      const u32 k1 = min(k0 + KC, K);
+#pragma unroll 1
+      for (u32 k = k0; k < k1; ++k) {
+        Raw r = next;
+        load(next, k + 2 < K);
+        if (left == 0) {
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+              for (int p = 0; p < 3; ++p) s[i][j][p].carry(hb, q, mh);
+          left = period;
+        }
+        --left;
+        if (weighted) {
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            const ulong2 f = factor[part == 0 ? row[i] - wg_m : a.decay_by_k ? k - k0 : KC - 1 - (k - k0) + (row[i] - wg_m)];
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+              u64 v = r.a[i][p] * f.x - mulhi64(r.a[i][p], f.y) * q;  // (the companion is at most one too small: below 3q)
+              v = v >= 2 * q ? v - 2 * q : v;
+              r.a[i][p] = v >= q ? v - q : v;
+            }
+          }
+        }
+        if (causal && !weighted) {  // (weighted: a factor of zero)
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) r.a[i][p] = (int64_t)k <= (int64_t)row[i] + off ? r.a[i][p] : 0;
+        }
+        Half bh[NT][2];
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int p = 0; p < 2; ++p) bh[i][p] = halves(r.b[i][p], hb);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const Half h0 = halves(r.a[i][0], hb), h1 = halves(r.a[i][1], hb);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            s[i][j][0].mac(h0, bh[j][0]);
+            s[i][j][1].mac(h0, bh[j][1]);
+            s[i][j][1].mac(h1, bh[j][0]);
+            s[i][j][2].mac(h1, bh[j][1]);
+          }
+        }
+      }
     }
   }
-  const u32 K2 = a.causal ? (u32)min((int64_t)a.t2.K, max(last + 1, (int64_t)0)) : a.t2.K;
-  if (K2) {
-    const ulong3 v = term(a.t2, K2, a.decay != nullptr);
-    r[0] = add_mod(r[0], v.x, q);
-    r[1] = add_mod(r[1], v.y, q);
-    r[2] = add_mod(r[2], v.z, q);
-  }
-  if (a.base.d) {
-    const u64* s = reb(c, a.base.d, rep) + h * a.base.head + m * a.base.row + j * a.base.col + off;
-    const u64 g = a.keep ? signed_mod(reb(c, a.keep, rep)[h], q, mh) : 1;
-    for (int p = 0; p < 2; ++p) r[p] = add_mod(r[p], a.keep ? mul_mod(s[p * a.base.comp], g, P) : s[p * a.base.comp], q);
-  }
-  u64* y = reb(c, a.out.d, rep) + h * a.out.head + m * a.out.row + j * a.out.col + off;
-  for (int p = 0; p < 3; ++p) y[p * a.out.comp] = r[p];
+  u64* y = reb(c, a.out.d, rep) + h * a.out.head + limb;
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+      if (m0 + i < a.M && j0 + j < a.Nn && n < c.N && (!a.skip_above || (int64_t)(j0 + j) <= (int64_t)(m0 + i) + off))
+#pragma unroll
+        for (int p = 0; p < 3; ++p) *(GLOBAL u64*)((GLOBAL char*)uniform(y + row[i] * a.out.row + col[j] * a.out.col + p * a.out.comp) + at) = s[i][j][p].template value<WIDE>(hb, P);
+}
+
+template <int MT, int NT, int WM, int WN, bool WIDE>
+static void launch_tiles(const DevCtx& c, const LinattnArgs& a, hipStream_t s) {
+  const u32 n_blocks = (c.N + 63) / 64, m_tiles = (a.M + MT * WM - 1) / (MT * WM), n_tiles = (a.Nn + NT * WN - 1) / (NT * WN);
+  hipLaunchKernelGGL((linattn_kernel<MT, NT, WM, WN, WIDE>), dim3(n_blocks * m_tiles * n_tiles * a.n_heads, a.n_limbs, c.nrep), dim3(64 * WM * WN), 0, s, c, a,
+                     n_blocks, m_tiles, n_tiles);
 }
 
 void launch_linattn(const DevCtx& c, const LinattnArgs& a, hipStream_t s) {
-  const u32 n_blocks = (c.N + 255) / 256;
-  hipLaunchKernelGGL(linattn_kernel, dim3(n_blocks * a.Nn * a.M * a.n_heads, a.n_limbs, c.nrep), dim3(256), 0, s, c, a, n_blocks);
+  if (!a.wide_primes) launch_tiles<1, 1, 1, 1, false>(c, a, s);
+  else if (a.M == 1)  launch_tiles<1, 4, 1, 4, true>(c, a, s);
+  else                launch_tiles<2, 4, 2, 2, true>(c, a, s);
 }
 
 }  // namespace acehip
