@@ -78,7 +78,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linattn_kernel(DevCtx c, Lina
   const int64_t off = a.off;
   // last column / key that the rows of the workgroup and of this wave see (rows past M: the last one's)
   const int64_t wg_last = (int64_t)min(wg_m + MT * WM, a.M) - 1 + off, last = (int64_t)min(m0 + MT, a.M) - 1 + off;
-  if (a.skip_above && (int64_t)((t % n_tiles) * (NT * WN)) > wg_last) return;
+  if (a.skip_above && (int64_t)j0 > last) return;  // (scores: no factors, so no barrier to meet)
   const DevPrime P = c.primes[gi];
   const u64 q = P.q, mh = P.prec128_hi;
   const u32 hb = (P.nbits + 1) / 2;
@@ -226,6 +226,198 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linattn_kernel(DevCtx c, Lina
         for (int p = 0; p < 3; ++p) *(GLOBAL u64*)((GLOBAL char*)uniform(y + row[i] * a.out.row + col[j] * a.out.col + p * a.out.comp) + at) = s[i][j][p].template value<WIDE>(hb, P);
 }
 
+// The same for larger products, with the operands of a workgroup's waves shared through LDS: every row of A and column of B is read by one wave,
+// has its factor and mask applied and its residues split in halves there, KS terms at a time and one stage ahead.
+__device__ __forceinline__ void lds_barrier() {  // LDS writes are visible, requests to memory stay in flight
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+template <int MT, int NT, int WM, int WN, int KS, int MIN_WAVES>
+__global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void linattn_shared_kernel(DevCtx c, LinattnArgs a, u32 n_blocks, u32 m_tiles, u32 n_tiles) {
+  constexpr u32 M = MT * WM, N = NT * WN, W = WM * WN, R = (M + N) / W;  // rows and columns of the workgroup's tile; its waves; rows that a wave stages
+  static_assert((M + N) % W == 0, "the waves stage equal shares");
+  constexpr u32 KC = 64;  // terms whose factors are prepared at a time
+  __shared__ uint4 operand[2][KS][M + N][64];  // halves of both polynomials: {l0, h0, l1, h1} of A's rows, then of B's columns
+  __shared__ ulong2 factor[KC + M];
+  u32 b = blockIdx.x;
+  const u32 groups = gridDim.x / (m_tiles * n_tiles);
+  u32 g, t;
+  if ((groups & 7u) == 0) {
+    const u32 x = b >> 3;
+    t = x % (m_tiles * n_tiles);
+    g = (x / (m_tiles * n_tiles)) * 8 + (b & 7u);
+  } else {
+    t = b % (m_tiles * n_tiles);
+    g = b / (m_tiles * n_tiles);
+  }
+  t = __builtin_amdgcn_readfirstlane(t);
+  g = __builtin_amdgcn_readfirstlane(g);
+  const u32 nb = g % n_blocks, h = g / n_blocks, rep = c.rep0 + blockIdx.z;
+  const u32 lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const u32 wg_m = (t / n_tiles) * M, wg_j = (t % n_tiles) * N;
+  const u32 wm = (wave / WN) * MT, wn = (wave % WN) * NT, m0 = wg_m + wm, j0 = wg_j + wn;
+  const u32 pos = a.pos0 + blockIdx.y, gi = limb_prime(pos, a.level, c.L);
+  if (!owns(c, gi)) return;
+  const int64_t off = a.off;
+  // last column / key that the rows of the workgroup and of this wave's results see (rows past M: the last one's)
+  const int64_t wg_last = (int64_t)min(wg_m + M, a.M) - 1 + off, last = (int64_t)min(m0 + MT, a.M) - 1 + off;
+  if (a.skip_above && (int64_t)wg_j > wg_last) return;
+  const bool idle = m0 >= a.M || j0 >= a.Nn || (a.skip_above && (int64_t)j0 > last);  // stages operands for the others
+  const DevPrime P = c.primes[gi];
+  const u64 q = P.q, mh = P.prec128_hi;
+  const u32 hb = (P.nbits + 1) / 2;
+  const u32 n = nb * 64 + lane, at = 8 * n;
+  const u64 limb = (u64)pos * c.N;
+  auto read = [&](const u64* p) { return *(const GLOBAL u64*)(uniform(p) + at); };
+
+  Acc s[MT][NT][3];
+  const u32 period = 1u << min(62 - P.nbits, 24u);
+  u32 left = period;  // terms that the sums still take
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int p = 0; p < 3; ++p) s[i][j][p] = Acc{0, 0, 0};
+  if (a.base.d) {  // one term: keep * base
+    const u64* S = reb(c, a.base.d, rep) + h * a.base.head + limb;
+    const Half f = halves(a.keep ? signed_mod(reb(c, a.keep, rep)[h], q, mh) : 1, hb);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+          s[i][j][p].mac(halves(read(S + min(m0 + i, a.M - 1) * a.base.row + min(j0 + j, a.Nn - 1) * a.base.col + p * a.base.comp), hb), f);
+    --left;
+  }
+  u32 buf = 0;
+#pragma unroll 1
+  for (u32 part = 0; part < 2; ++part) {
+    const LinattnTerm& t = part ? a.t2 : a.t1;
+    const bool causal = part && a.causal, weighted = part ? a.decay != nullptr : a.scale != nullptr;
+    const u32 K = causal ? (u32)min((int64_t)t.K, max(wg_last + 1, (int64_t)0)) : t.K;  // of the workgroup; K_own: of this wave's results
+    const u32 K_own = idle ? 0 : causal ? (u32)min((int64_t)t.K, max(last + 1, (int64_t)0)) : t.K;
+    if (K == 0) continue;
+    const u64* A = reb(c, t.a.d, rep) + (h / t.a_group) * t.a.head + limb;
+    const u64* B = reb(c, t.b.d, rep) + (h / t.b_group) * t.b.head + limb;
+    // the wave's share: row wave + r*W of the tile's rows, then columns
+    const u64* from[R];
+    u64 next[R], comp[R];
+#pragma unroll
+    for (u32 r = 0; r < R; ++r) {
+      const u32 x = wave + r * W;
+      from[r] = x < M ? A + min(wg_m + x, a.M - 1) * t.a.row : B + min(wg_j + x - M, a.Nn - 1) * t.b.col;
+      next[r] = x < M ? t.a.col : t.b.row;
+      comp[r] = x < M ? t.a.comp : t.b.comp;
+    }
+    u64 raw[KS][R][2];
+    auto load = [&](u32 k0) {  // (terms past the last are read again, and staged as zeros)
+#pragma unroll
+      for (int e = 0; e < KS; ++e) {
+        const u64 k = min(k0 + e, K - 1);
+#pragma unroll
+        for (u32 r = 0; r < R; ++r)
+#pragma unroll
+          for (int p = 0; p < 2; ++p) raw[e][r][p] = read(from[r] + k * next[r] + p * comp[r]);
+      }
+    };
+    auto factors = [&](u32 k0) {  // of the terms from k0 on, as in linattn_kernel
+      lds_barrier();
+      for (u32 e = threadIdx.x; e < KC + M; e += 64 * W) {
+        const int64_t d = part == 0 ? (int64_t)min(wg_m + e, a.M - 1) : a.decay_by_k ? (int64_t)t.K - 1 - k0 - e : (int64_t)wg_m + off - (k0 + KC - 1) + e;
+        const bool there = d >= 0 && d < (int64_t)(part ? t.K : a.M);
+        const u64 f = there ? signed_mod(part ? reb(c, a.decay, rep)[h * a.decay_ld + d] : reb(c, a.scale, rep)[h * a.M + d], q, mh) : 0;
+        factor[e] = ulong2{f, f * mh + mulhi64(f, P.prec128_lo)};
+      }
+      lds_barrier();
+    };
+    auto stage = [&](u32 k0, u32 to) {
+#pragma unroll
+      for (int e = 0; e < KS; ++e) {
+        const u32 k = k0 + e;
+#pragma unroll
+        for (u32 r = 0; r < R; ++r) {
+          const u32 x = wave + r * W, mask = (1u << hb) - 1;
+          u64 v[2] = {raw[e][r][0], raw[e][r][1]};
+          bool there = true;
+          if (x < M) {
+            const u32 m = min(wg_m + x, a.M - 1);
+            there = (int64_t)k < (causal ? min((int64_t)K, (int64_t)m + off + 1) : (int64_t)K);
+            if (weighted) {
+              const u32 kc = k % KC;
+              const ulong2 f = factor[part == 0 ? m - wg_m : a.decay_by_k ? kc : KC - 1 - kc + (m - wg_m)];
+#pragma unroll
+              for (int p = 0; p < 2; ++p) {
+                v[p] = v[p] * f.x - mulhi64(v[p], f.y) * q;  // (the companion is at most one too small: below 3q)
+                v[p] = v[p] >= 2 * q ? v[p] - 2 * q : v[p];
+                v[p] = v[p] >= q ? v[p] - q : v[p];
+              }
+            }
+          }
+          operand[to][e][x][lane] = there ? uint4{(u32)v[0] & mask, (u32)(v[0] >> hb), (u32)v[1] & mask, (u32)(v[1] >> hb)} : uint4{0, 0, 0, 0};
+        }
+      }
+    };
+    load(0);
+    if (weighted) factors(0);
+    else          lds_barrier();  // (the part before has read its last operands)
+    stage(0, buf);
+    load(KS);
+#pragma unroll 1
+    for (u32 k0 = 0; k0 < K; k0 += KS) {
+      if (weighted && (k0 + KS) % KC == 0 && k0 + KS < K) factors(k0 + KS);
+      else                                                lds_barrier();
+      if (k0 + KS < K) {
+        stage(k0 + KS, buf ^ 1u);
+        load(k0 + 2 * KS);
+      }
+#pragma unroll
+      for (int e = 0; e < KS; ++e) {
+        if (k0 + e >= K_own) continue;
+        if (left == 0) {
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+              for (int p = 0; p < 3; ++p) s[i][j][p].carry(hb, q, mh);
+          left = period;
+        }
+        --left;
+        uint4 xa[MT], xb[NT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) xa[i] = operand[buf][e][wm + i][lane];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) xb[j] = operand[buf][e][M + wn + j][lane];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const Half h0{xa[i].x, xa[i].y, xa[i].x + xa[i].y}, h1{xa[i].z, xa[i].w, xa[i].z + xa[i].w};
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const Half b0{xb[j].x, xb[j].y, xb[j].x + xb[j].y}, b1{xb[j].z, xb[j].w, xb[j].z + xb[j].w};
+            s[i][j][0].mac(h0, b0);
+            s[i][j][1].mac(h0, b1);
+            s[i][j][1].mac(h1, b0);
+            s[i][j][2].mac(h1, b1);
+          }
+        }
+      }
+      buf ^= 1u;
+    }
+  }
+  u64* y = reb(c, a.out.d, rep) + h * a.out.head + limb;
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+      if (m0 + i < a.M && j0 + j < a.Nn && (!a.skip_above || (int64_t)(j0 + j) <= (int64_t)(m0 + i) + off))
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+          *(GLOBAL u64*)((GLOBAL char*)uniform(y + (m0 + i) * a.out.row + (j0 + j) * a.out.col + p * a.out.comp) + at) = s[i][j][p].template value<true>(hb, P);
+}
+
 template <int MT, int NT, int WM, int WN, bool WIDE>
 static void launch_tiles(const DevCtx& c, const LinattnArgs& a, hipStream_t s) {
   const u32 n_blocks = (c.N + 63) / 64, m_tiles = (a.M + MT * WM - 1) / (MT * WM), n_tiles = (a.Nn + NT * WN - 1) / (NT * WN);
@@ -233,10 +425,21 @@ static void launch_tiles(const DevCtx& c, const LinattnArgs& a, hipStream_t s) {
                      n_blocks, m_tiles, n_tiles);
 }
 
+template <int MT, int NT, int WM, int WN, int KS, int MIN_WAVES>
+static void launch_shared(const DevCtx& c, const LinattnArgs& a, hipStream_t s) {
+  const u32 n_blocks = c.N / 64, m_tiles = (a.M + MT * WM - 1) / (MT * WM), n_tiles = (a.Nn + NT * WN - 1) / (NT * WN);
+  hipLaunchKernelGGL((linattn_shared_kernel<MT, NT, WM, WN, KS, MIN_WAVES>), dim3(n_blocks * m_tiles * n_tiles * a.n_heads, a.n_limbs, c.nrep), dim3(64 * WM * WN), 0, s, c,
+                     a, n_blocks, m_tiles, n_tiles);
+}
+
 void launch_linattn(const DevCtx& c, const LinattnArgs& a, hipStream_t s) {
   if (!a.wide_primes) launch_tiles<1, 1, 1, 1, false>(c, a, s);
   else if (a.M == 1)  launch_tiles<1, 4, 1, 4, true>(c, a, s);
-  else                launch_tiles<2, 4, 2, 2, true>(c, a, s);
+  else if (c.N >= 64 && a.M > 4 && a.Nn > 4 && a.t1.K + a.t2.K >= 8) {
+    launch_shared<2, 2, 2, 2, 2, 4>(c, a, s);
+  } else {
+    launch_tiles<2, 4, 2, 2, true>(c, a, s);
+  }
 }
 
 }  // namespace acehip
