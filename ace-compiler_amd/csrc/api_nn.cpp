@@ -30,9 +30,12 @@ struct Call {
     if (pos0 > level + c->hp.K || n_limbs > level + c->hp.K - pos0) return bad("limb range exceeds level + K");
     return ACEHIP_OK;
   }
+  // every prime of the call is above 2^bits and up to 2^64 / 9 (all but those of chosen test chains)
   bool primes_above(u32 bits) const {
-    for (u32 p = pos0; p < pos0 + n_limbs; ++p)
-      if (c->hp.q(limb_prime(p, level, c->hp.L)) >> bits == 0) return false;
+    for (u32 p = pos0; p < pos0 + n_limbs; ++p) {
+      const u64 q = c->hp.q(limb_prime(p, level, c->hp.L));
+      if (q >> bits == 0 || q > ~0ull / 9) return false;
+    }
     return true;
   }
   int view(View& v, const acehip_mat* a, u64 heads, u64 rows, u64 cols, u64 comps) const {

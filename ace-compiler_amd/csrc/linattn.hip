@@ -15,6 +15,29 @@ __device__ __forceinline__ Half halves(u64 x, u32 hb) {
   const u32 l = (u32)x & ((1u << hb) - 1), h = (u32)(x >> hb);
   return Half{l, h, l + h};
 }
+// What the sums of one prime need.  WIDE: primes above 2^32 and up to 2^64 / 9.
+template <bool WIDE>
+struct Reduce {
+  u64 q, nq, mh, ml;   // the prime, its negative, floor(2^128 / q)
+  u64 w, wp;           // 2^(2 hb) mod q and its companion, at most two units of 2^-64 too small
+  double per_q;        // 2^32 / q
+  float near_q;        // the same, a little too small
+  u32 hb, mask;
+  __device__ __forceinline__ explicit Reduce(const DevPrime& P) : q(P.q), nq(0 - P.q), mh(P.prec128_hi), ml(P.prec128_lo) {
+    hb = (P.nbits + 1) / 2;
+    mask = (1u << hb) - 1;
+    w = signed_mod(1ll << (2 * hb), q, mh);
+    wp = w * mh + mulhi64(w, ml);
+    per_q = 4294967296.0 / (double)q;
+    near_q = (float)per_q * 0.999999f;
+  }
+};
+// a * w mod q up to multiples of q: below 5q for any a, with a companion wp of w that is at most two units of 2^-64 too small (the quotient leaves
+// out the low product and two carries)
+__device__ __forceinline__ u64 mul_near(u64 a, u64 w, u64 wp, u64 nq) {
+  const u64 h = (u64)(u32)(a >> 32) * (u32)(wp >> 32) + __umulhi((u32)(a >> 32), (u32)wp) + __umulhi((u32)a, (u32)(wp >> 32));
+  return a * w + h * nq;
+}
 struct Acc {
   u64 ll, mm, hh;
   __device__ __forceinline__ void mac(const Half& x, const Half& y) {
@@ -22,23 +45,29 @@ struct Acc {
     mm += (u64)x.s * y.s;
     hh += (u64)x.h * y.h;
   }
+  // carries brought up and hh reduced below 3q (2q at primes of over 40 bits): room for as many terms again
   template <bool WIDE>
-  __device__ __forceinline__ u64 value(u32 hb, const DevPrime& P) const {
-    unsigned __int128 v = ll;
-    v += (unsigned __int128)(mm - ll - hh) << hb;
-    v += (unsigned __int128)hh << (2 * hb);
-    const U128 x{(u64)v, (u64)(v >> 64)};
-    return WIDE ? reduce128(x, P.q, P.prec128_lo, (u32)P.prec128_hi) : reduce128_generic(x, P.q, P.prec128_lo, P.prec128_hi);
-  }
-  // carries brought up and hh reduced below 2q: room for as many terms again
-  __device__ __forceinline__ void carry(u32 hb, u64 q, u64 mh) {
-    const u64 mask = (1ull << hb) - 1;
-    u64 mid = mm - ll - hh + (ll >> hb);
-    ll &= mask;
-    hh += mid >> hb;
-    mid &= mask;
-    hh -= mulhi64(hh, mh) * q;
+  __device__ __forceinline__ void carry(const Reduce<WIDE>& r) {
+    u64 mid = mm - ll - hh + (ll >> r.hb);
+    ll = (u32)ll & r.mask;
+    hh += mid >> r.hb;
+    mid = (u32)mid & r.mask;
+    if (WIDE) hh += (u64)(u32)((double)(u32)(hh >> 32) * r.per_q) * r.nq;
+    else      hh -= mulhi64(hh, r.mh) * r.q;
     mm = mid + ll + hh;
+  }
+  template <bool WIDE>
+  __device__ __forceinline__ u64 value(const Reduce<WIDE>& r) const {
+    const u64 mid = mm - ll - hh + (ll >> r.hb);
+    if (!WIDE) {
+      const unsigned __int128 v = ((unsigned __int128)hh << (2 * r.hb)) + ((unsigned __int128)mid << r.hb) + ((u32)ll & r.mask);
+      return reduce128_generic(U128{(u64)v, (u64)(v >> 64)}, r.q, r.ml, r.mh);
+    }
+    // low part below 2^(2 hb) <= 4q, the rest times 2^(2 hb) below 5q; then the quotient, below 9, from single precision: not too large, at most
+    // one too small
+    const u64 v = mul_near(hh + (mid >> r.hb), r.w, r.wp, r.nq) + (((u64)((u32)mid & r.mask) << r.hb) | ((u32)ll & r.mask));
+    const u64 x = v + (u64)(u32)((float)(u32)(v >> 32) * r.near_q) * r.nq;
+    return x >= r.q ? x - r.q : x;
   }
 };
 
@@ -80,8 +109,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linattn_kernel(DevCtx c, Lina
   const int64_t wg_last = (int64_t)min(wg_m + MT * WM, a.M) - 1 + off, last = (int64_t)min(m0 + MT, a.M) - 1 + off;
   if (a.skip_above && (int64_t)j0 > last) return;  // (scores: no factors, so no barrier to meet)
   const DevPrime P = c.primes[gi];
+  const Reduce<WIDE> red(P);
   const u64 q = P.q, mh = P.prec128_hi;
-  const u32 hb = (P.nbits + 1) / 2;
+  const u32 hb = red.hb;
   const u32 n = nb * 64 + lane, at = 8 * min(n, c.N - 1);  // (rings below 64: the lanes behind the ring repeat its last coefficient and store nothing)
   const u64 limb = (u64)pos * c.N;
   u32 row[MT], col[NT];
@@ -175,7 +205,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linattn_kernel(DevCtx c, Lina
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
-              for (int p = 0; p < 3; ++p) s[i][j][p].carry(hb, q, mh);
+              for (int p = 0; p < 3; ++p) s[i][j][p].carry(red);
           left = period;
         }
         --left;
@@ -223,7 +253,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linattn_kernel(DevCtx c, Lina
     for (int j = 0; j < NT; ++j)
       if (m0 + i < a.M && j0 + j < a.Nn && n < c.N && (!a.skip_above || (int64_t)(j0 + j) <= (int64_t)(m0 + i) + off))
 #pragma unroll
-        for (int p = 0; p < 3; ++p) *(GLOBAL u64*)((GLOBAL char*)uniform(y + row[i] * a.out.row + col[j] * a.out.col + p * a.out.comp) + at) = s[i][j][p].template value<WIDE>(hb, P);
+        for (int p = 0; p < 3; ++p) *(GLOBAL u64*)((GLOBAL char*)uniform(y + row[i] * a.out.row + col[j] * a.out.col + p * a.out.comp) + at) = s[i][j][p].value(red);
 }
 
 // The same for larger products, with the operands of a workgroup's waves shared through LDS: every row of A and column of B is read by one wave,
@@ -265,8 +295,9 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void linattn_shared_kernel
   if (a.skip_above && (int64_t)wg_j > wg_last) return;
   const bool idle = m0 >= a.M || j0 >= a.Nn || (a.skip_above && (int64_t)j0 > last);  // stages operands for the others
   const DevPrime P = c.primes[gi];
+  const Reduce<true> red(P);
   const u64 q = P.q, mh = P.prec128_hi;
-  const u32 hb = (P.nbits + 1) / 2;
+  const u32 hb = red.hb;
   const u32 n = nb * 64 + lane, at = 8 * n;
   const u64 limb = (u64)pos * c.N;
   auto read = [&](const u64* p) { return *(const GLOBAL u64*)(uniform(p) + at); };
@@ -303,24 +334,28 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void linattn_shared_kernel
     const u64* A = reb(c, t.a.d, rep) + (h / t.a_group) * t.a.head + limb;
     const u64* B = reb(c, t.b.d, rep) + (h / t.b_group) * t.b.head + limb;
     // the wave's share: row wave + r*W of the tile's rows, then columns
-    const u64* from[R];
-    u64 next[R], comp[R];
+    const u64* from[R][2];
+    u64 next[R];
 #pragma unroll
     for (u32 r = 0; r < R; ++r) {
       const u32 x = wave + r * W;
-      from[r] = x < M ? A + min(wg_m + x, a.M - 1) * t.a.row : B + min(wg_j + x - M, a.Nn - 1) * t.b.col;
+      from[r][0] = x < M ? A + min(wg_m + x, a.M - 1) * t.a.row : B + min(wg_j + x - M, a.Nn - 1) * t.b.col;
+      from[r][1] = from[r][0] + (x < M ? t.a.comp : t.b.comp);
       next[r] = x < M ? t.a.col : t.b.row;
-      comp[r] = x < M ? t.a.comp : t.b.comp;
     }
     u64 raw[KS][R][2];
-    auto load = [&](u32 k0) {  // (terms past the last are read again, and staged as zeros)
+    u32 k_load = 0;
+    auto load = [&] {  // the next KS terms (behind the last one it is read again, and staged as zeros)
 #pragma unroll
       for (int e = 0; e < KS; ++e) {
-        const u64 k = min(k0 + e, K - 1);
+        const bool more = ++k_load < K;
 #pragma unroll
         for (u32 r = 0; r < R; ++r)
 #pragma unroll
-          for (int p = 0; p < 2; ++p) raw[e][r][p] = read(from[r] + k * next[r] + p * comp[r]);
+          for (int p = 0; p < 2; ++p) {
+            raw[e][r][p] = read(from[r][p]);
+            from[r][p] += more ? next[r] : 0;
+          }
       }
     };
     auto factors = [&](u32 k0) {  // of the terms from k0 on, as in linattn_kernel
@@ -339,12 +374,13 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void linattn_shared_kernel
         const u32 k = k0 + e;
 #pragma unroll
         for (u32 r = 0; r < R; ++r) {
-          const u32 x = wave + r * W, mask = (1u << hb) - 1;
+          const u32 x = wave + r * W;
           u64 v[2] = {raw[e][r][0], raw[e][r][1]};
-          bool there = true;
+          u32 mask = red.mask, there = ~0u;
           if (x < M) {
             const u32 m = min(wg_m + x, a.M - 1);
-            there = (int64_t)k < (causal ? min((int64_t)K, (int64_t)m + off + 1) : (int64_t)K);
+            there = (int64_t)k < (causal ? min((int64_t)K, (int64_t)m + off + 1) : (int64_t)K) ? ~0u : 0;
+            mask &= there;
             if (weighted) {
               const u32 kc = k % KC;
               const ulong2 f = factor[part == 0 ? m - wg_m : a.decay_by_k ? kc : KC - 1 - kc + (m - wg_m)];
@@ -356,22 +392,22 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void linattn_shared_kernel
               }
             }
           }
-          operand[to][e][x][lane] = there ? uint4{(u32)v[0] & mask, (u32)(v[0] >> hb), (u32)v[1] & mask, (u32)(v[1] >> hb)} : uint4{0, 0, 0, 0};
+          operand[to][e][x][lane] = uint4{(u32)v[0] & mask, (u32)(v[0] >> hb) & there, (u32)v[1] & mask, (u32)(v[1] >> hb) & there};
         }
       }
     };
-    load(0);
+    load();
     if (weighted) factors(0);
     else          lds_barrier();  // (the part before has read its last operands)
     stage(0, buf);
-    load(KS);
+    load();
 #pragma unroll 1
     for (u32 k0 = 0; k0 < K; k0 += KS) {
       if (weighted && (k0 + KS) % KC == 0 && k0 + KS < K) factors(k0 + KS);
       else                                                lds_barrier();
       if (k0 + KS < K) {
         stage(k0 + KS, buf ^ 1u);
-        load(k0 + 2 * KS);
+        load();
       }
 #pragma unroll
       for (int e = 0; e < KS; ++e) {
@@ -382,7 +418,7 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void linattn_shared_kernel
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
-              for (int p = 0; p < 3; ++p) s[i][j][p].carry(hb, q, mh);
+              for (int p = 0; p < 3; ++p) s[i][j][p].carry(red);
           left = period;
         }
         --left;
@@ -415,7 +451,7 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void linattn_shared_kernel
       if (m0 + i < a.M && j0 + j < a.Nn && (!a.skip_above || (int64_t)(j0 + j) <= (int64_t)(m0 + i) + off))
 #pragma unroll
         for (int p = 0; p < 3; ++p)
-          *(GLOBAL u64*)((GLOBAL char*)uniform(y + (m0 + i) * a.out.row + (j0 + j) * a.out.col + p * a.out.comp) + at) = s[i][j][p].template value<true>(hb, P);
+          *(GLOBAL u64*)((GLOBAL char*)uniform(y + (m0 + i) * a.out.row + (j0 + j) * a.out.col + p * a.out.comp) + at) = s[i][j][p].value(red);
 }
 
 template <int MT, int NT, int WM, int WN, bool WIDE>
@@ -436,7 +472,7 @@ void launch_linattn(const DevCtx& c, const LinattnArgs& a, hipStream_t s) {
   if (!a.wide_primes) launch_tiles<1, 1, 1, 1, false>(c, a, s);
   else if (a.M == 1)  launch_tiles<1, 4, 1, 4, true>(c, a, s);
   else if (c.N >= 64 && a.M > 4 && a.Nn > 4 && a.t1.K + a.t2.K >= 8) {
-    launch_shared<2, 2, 2, 2, 2, 4>(c, a, s);
+    launch_shared<2, 2, 2, 2, 1, 4>(c, a, s);
   } else {
     launch_tiles<2, 4, 2, 2, true>(c, a, s);
   }

@@ -73,7 +73,7 @@ struct LinattnArgs {
   int32_t off = 0;
   u32 causal = 0, decay_by_k = 0, skip_above = 0;
   u32 level, pos0, n_limbs;
-  bool wide_primes = false;        // every prime of the call is above 2^32
+  bool wide_primes = false;        // every prime of the call is above 2^32 and up to 2^64 / 9
 };
 void launch_linattn(const DevCtx& c, const LinattnArgs& a, hipStream_t s);
 
