@@ -646,3 +646,194 @@ def test_sharded_context_computes_its_limbs(contexts):
     for b in (base, dw):
         b.free()
     rt.close()
+
+
+# ---- used together: a layer on encrypted data ------------------------------------------------------------------------------------------
+class Client:
+    """A CKKS user on top of the C ABI: secret and relinearisation key, encryption, decryption and decoding in whole numbers on the host
+    (transforms on the device)."""
+
+    def __init__(self, rt, seed):
+        self.rt, self.rng = rt, np.random.default_rng(seed)
+        self.N, self.q = rt.N, np.array(rt.primes, dtype=object)[:, None]
+        self.full = list(range(rt.L + rt.K))
+        self.s = self.ntt(self.rng.integers(-1, 2, self.N).astype(object), self.full)
+        s2 = self.s * self.s % self.q
+        P = int(np.prod(self.q[rt.L:, 0]))
+        key = []
+        for d in range(rt.dnum):
+            a = self.uniform(self.full)
+            own = np.array([[P % int(self.q[i, 0]) if i < rt.L and i // rt.alpha == d else 0] for i in self.full], dtype=object)
+            key += [(self.noise(self.full) - a * self.s + own * s2) % self.q, a]
+        self.key = dev(rt, np.stack(key).astype(np.uint64))
+        j = np.array([pow(5, int(k), 2 * self.N) for k in range(self.N // 2)])
+        self.decode_matrix = np.exp(1j * np.pi * (j[:, None] * np.arange(self.N)[None] % (2 * self.N)) / self.N)
+
+    def ntt(self, coefficients, limbs):
+        return self.rt.ntt((coefficients[None] % self.q[limbs]).astype(np.uint64), self.rt.L, pos0=limbs[0]).astype(object)
+
+    def uniform(self, limbs):
+        return np.stack([self.rng.integers(0, int(self.q[i, 0]), self.N, dtype=np.uint64) for i in limbs]).astype(object)
+
+    def noise(self, limbs):
+        return self.ntt(np.rint(self.rng.normal(0, 3.2, self.N)).astype(np.int64).astype(object), limbs)
+
+    def encrypt(self, message, level):
+        limbs = list(range(level))
+        m = self.rt.encode(np.asarray(message, dtype=np.float64), level)[0].astype(object)
+        a = self.uniform(limbs)
+        return np.stack([(m + self.noise(limbs) - a * self.s[:level]) % self.q[:level], a]).astype(np.uint64)
+
+    def decrypt(self, ct, scale):
+        """ct: [2][level][N]"""
+        m = (ct[0, :1].astype(object) + ct[1, :1].astype(object) * self.s[:1]) % self.q[:1]
+        c = self.rt.ntt(m.astype(np.uint64), self.rt.L, inverse=True)[0].astype(object)
+        c = np.where(c > self.q[0] // 2, c - self.q[0], c).astype(np.float64) / scale
+        return (self.decode_matrix @ c).real
+
+
+class Cts:
+    """device array of ciphertexts [heads][rows][cols][comps], limbs of `level`, with their scale"""
+
+    def __init__(self, rt, shape, level, scale, data=None):
+        self.rt, self.shape, self.level, self.scale = rt, shape, level, scale
+        self.poly = level * rt.N
+        self.buf = rt.to_device(data) if data is not None else rt.buf(int(np.prod(shape)) * self.poly)
+
+    def strides(self):
+        h, r, c, p = self.shape
+        return dict(head=r * c * p * self.poly, row=c * p * self.poly, col=p * self.poly, comp=self.poly)
+
+    def mat(self, **other):
+        return self.rt.mat(self.buf.ptr, **{**self.strides(), **other})
+
+    def at(self, i, p):
+        return self.buf.ptr + 8 * self.poly * (i * self.shape[3] + p)
+
+    def finish(self, client, times):
+        """relinearised where there are three polynomials, then rescaled `times` times"""
+        rt, lib, N = self.rt, self.rt.lib, self.rt.N
+        n = int(np.prod(self.shape[:3]))
+        out = Cts(rt, (*self.shape[:3], 2), self.level - times, self.scale / float(np.prod([float(rt.primes[self.level - 1 - t]) for t in range(times)])))
+        t = [rt.buf(self.poly) for _ in range(6)]
+        for i in range(n):
+            c = [self.at(i, 0), self.at(i, 1)]
+            if self.shape[3] == 3:
+                rt.check(lib.acehip_key_switch(rt.h, t[0].ptr, t[1].ptr, self.at(i, 2), client.key.ptr, self.level, None))
+                for p in (0, 1):
+                    rt.check(lib.acehip_modadd(rt.h, t[p].ptr, t[p].ptr, c[p], self.level, 0, self.level, None))
+                c = [t[0].ptr, t[1].ptr]
+            for k in range(times):
+                to = [out.at(i, 0), out.at(i, 1)] if k == times - 1 else [t[2 + 2 * (k % 2)].ptr, t[3 + 2 * (k % 2)].ptr]
+                rt.check(lib.acehip_rescale2(rt.h, to[0], to[1], c[0], c[1], self.level - k, None))
+                c = to
+        rt.sync()
+        for b in (*t, self.buf):
+            b.free()
+        return out
+
+    def values(self, client):
+        d = self.buf.download((*self.shape, self.level, self.rt.N))
+        return np.array([[[client.decrypt(d[h, r, c], self.scale) for c in range(self.shape[2])] for r in range(self.shape[1])] for h in range(self.shape[0])])
+
+
+def test_layer_on_encrypted_data():
+    """Projections with int8 weights, rotary positions with two axes, causal linear attention over a chunk of two tokens, its state, a third token in
+    the recurrent form, output projection -- against the same layer in double precision on the messages.  A scale of 2^51 leaves errors of
+    2^-51 times noise (about 2^6 fresh, 2^12 from a key switch or a rescale in every slot) times values and weights of a few units through six levels:
+    below 2^-30; a wrong term is of the size of the values."""
+    rt = A.AceHip(1024, 7, 60, 51, 3)
+    cl = Client(rt, 11)
+    N, slots, delta = rt.N, rt.N // 2, 2.0**51
+    rng = np.random.default_rng(12)
+    H, dk, dv, din, T = 2, 4, 3, 5, 3
+    x = rng.uniform(-1, 1, (T, din, slots))
+    assert np.max(np.abs(cl.decrypt(cl.encrypt(x[0, 0], 3), delta) - x[0, 0])) < 2.0**-35
+    cx = Cts(rt, (1, T, din, 2), 7, delta, np.stack([[cl.encrypt(x[t, i], 7) for i in range(din)] for t in range(T)]))
+    d_x = cx
+
+    def project(src, w, scale, tok=None, shape=None):
+        """w * scale: rows of tokens -> [token][n_out]"""
+        n_out = w.shape[0]
+        mul = np.rint(scale * delta).astype(np.int64)
+        out = Cts(rt, shape or (1, T, n_out, 2), src.level, src.scale * delta * (delta if tok else 1))
+        dw, dm = dev(rt, w), dev(rt, mul)
+        rt.linear_i8(rt.mat(out.buf.ptr, row=n_out * 2 * out.poly, col=2 * out.poly, comp=out.poly), src.mat(), dw.ptr, w.shape[1], T, w.shape[1], n_out, 2, src.level,
+                     d_mul=dm.ptr, d_tok=tok.ptr if tok else None, tok_stride=out.poly)
+        rt.sync()
+        dw.free()
+        dm.free()
+        return out
+
+    wq, wk, wv = (rng.integers(-127, 128, (n, din)).astype(np.int8) for n in (H * dk, dk, dv))
+    sq, sk, sv = (rng.uniform(0.002, 0.008, n) for n in (H * dk, dk, dv))
+    keep_slot = rng.integers(0, 2, (T, slots)).astype(np.float64)      # tokens that are padding in some of the sequences
+    mask = dev(rt, np.stack([rt.encode(keep_slot[t], 7)[0] for t in range(T)]))
+    q = project(d_x, wq, sq, shape=(T, H, dk, 2)).finish(cl, 1)        # [token][head][feature]
+    k = project(d_x, wk, sk, shape=(T, 1, dk, 2)).finish(cl, 1)
+    v = project(d_x, wv, sv, tok=mask, shape=(T, 1, dv, 2)).finish(cl, 2)
+    xq = np.einsum("ji,tis->tjs", wq * sq[:, None], x).reshape(T, H, dk, slots)
+    xk, xv = np.einsum("ji,tis->tjs", wk * sk[:, None], x), np.einsum("ji,tis->tjs", wv * sv[:, None], x) * keep_slot[:, None]
+    assert np.max(np.abs(v.values(cl)[:, 0] - xv)) < 2.0**-30
+
+    # rotary positions: pair 0 by time, pair 1 by place; tables at the level of the queries, one for each token
+    pos = np.stack([np.repeat(np.arange(T) + 1000.0, slots), np.tile(np.arange(slots) % 7, T).astype(np.float64)])
+    freq, axis = [1.0, 0.1], [0, 1]
+    d_pos, d_cos, d_sin = dev(rt, pos), rt.buf(2 * T * slots, np.float64), rt.buf(2 * T * slots, np.float64)
+    rt.rope_messages(d_cos.ptr, d_sin.ptr, T * slots, d_pos.ptr, T * slots, T * slots, freq, axis, 2)
+    tables = []
+    for d in (d_cos, d_sin):
+        t = rt.buf(T * 2 * q.poly)
+        for tok, pair_i in itertools.product(range(T), range(2)):
+            rt.check(rt.lib.acehip_encode(rt.h, t.at((tok * 2 + pair_i) * q.poly), None, d.at(pair_i * T * slots + tok * slots), 1, slots, 0, delta, 1, q.level, 0, None))
+        tables.append(t)
+    ang = (pos[axis] * np.array(freq)[:, None]).reshape(2, T, slots).transpose(1, 0, 2)
+
+    def turn(ct, heads, val):
+        rt.rope(ct.mat(head=ct.strides()["row"], row=ct.strides()["head"]), ct.mat(head=ct.strides()["row"], row=ct.strides()["head"]), tables[0].ptr, tables[1].ptr, ct.poly,
+                2 * ct.poly, heads, T, dk, 2, ct.level)
+        ct.scale *= delta
+        a, b = val[..., :2, :], val[..., 2:, :]
+        c, s = (f(ang) if val.ndim == 3 else f(ang)[:, None] for f in (np.cos, np.sin))
+        return ct.finish(cl, 1), np.concatenate([a * c - b * s, a * s + b * c], axis=-2)
+
+    q, xq = turn(q, H, xq)
+    k, xk = turn(k, 1, xk)
+    tokens = lambda ct, first=0: rt.mat(ct.buf.ptr + 8 * first * ct.strides()["head"], head=ct.strides()["row"], row=ct.strides()["head"], col=ct.strides()["col"], comp=ct.poly)
+    assert np.max(np.abs(q.values(cl) - xq)) < 2.0**-30 and q.level == k.level == v.level == 5
+
+    # a chunk of two tokens
+    gamma = np.array([0.9, 0.75])
+    decay = np.rint(gamma[:, None] ** np.arange(2) * delta).astype(np.int64)
+    d_decay = dev(rt, decay)
+    p = Cts(rt, (H, 2, 2, 3), 5, q.scale * k.scale, np.zeros((H, 2, 2, 3, 5, N), np.uint64))
+    rt.linattn_scores(p.mat(), tokens(q), tokens(k), H, 1, 2, 2, dk, 5)
+    p = p.finish(cl, 1)
+    o = Cts(rt, (H, 2, dv, 3), 4, p.scale * v.scale * delta)
+    rt.linattn_out(o.mat(), None, None, p.mat(), tokens(v), H, 1, 2, 2, dk, dv, 4, d_decay=d_decay.ptr)
+    o = o.finish(cl, 2)
+    want = np.zeros((H, T, dv, slots))
+    for h, t in itertools.product(range(H), range(T)):
+        for s in range(t + 1):
+            want[h, t] += gamma[h] ** (t - s) * np.sum(xq[t, h] * xk[s], axis=0) * xv[s]
+    assert np.max(np.abs(o.values(cl) - want[:, :2])) < 2.0**-30
+
+    # its state, and the third token
+    S = Cts(rt, (H, dk, dv, 3), 5, k.scale * v.scale * delta)
+    rt.linattn_state(S.mat(), None, tokens(k), tokens(v), H, 1, 2, dk, dv, 5, d_decay=d_decay.ptr)
+    S = S.finish(cl, 2)
+    keep = dev(rt, np.rint(gamma * (k.scale * v.scale / S.scale)).astype(np.int64))
+    S1 = Cts(rt, (H, dk, dv, 3), 3, k.scale * v.scale)
+    rt.linattn_state(S1.mat(), S.mat(), tokens(k, 2), tokens(v, 2), H, 1, 1, dk, dv, 3, d_keep=keep.ptr)
+    S1 = S1.finish(cl, 1)
+    o1 = Cts(rt, (H, 1, dv, 3), 2, q.scale * S1.scale)
+    rt.linattn_out(o1.mat(), tokens(q, 2), S1.mat(), None, None, H, 1, 1, 0, dk, dv, 2)
+    o1 = o1.finish(cl, 1)
+    assert o1.level == 1 and np.max(np.abs(o1.values(cl)[:, 0] - want[:, 2])) < 2.0**-30
+
+    # output projection of the third token: heads and features as one row of inputs
+    wo = rng.integers(-3, 4, (4, H * dv)).astype(np.int8)
+    y, dw = Cts(rt, (1, 1, 4, 2), 1, o1.scale), dev(rt, wo)
+    rt.linear_i8(y.mat(), rt.mat(o1.buf.ptr, col=2 * o1.poly, comp=o1.poly), dw.ptr, H * dv, 1, H * dv, 4, 2, 1)
+    assert np.max(np.abs(y.values(cl)[0, 0] - wo @ want[:, 2].reshape(H * dv, slots))) < 2.0**-26
+    rt.close()
