@@ -6,8 +6,9 @@ namespace acehip {
 // Sums of products of residues, exact: the residues are split at hb = ceil(bits / 2), and the three 64-bit sums of
 //   x*y = ll + ((xl + xh)(yl + yh) - ll - hh) 2^hb + hh 2^(2 hb)
 // take one 32x32 multiply-add each.  mm may wrap on the way: only the difference mm - ll - hh counts.  For primes of n bits a product's
-// middle part is below 2^(n+1), and an accumulator takes at most two products a term, so 2^(62-n) terms stay below 2^64 (the exact bound
-// 2^(64-n) (2^hb - 1)(2^(n-hb) - 1) leaves room for what carry() leaves in the sums); then carry() makes room again.
+// middle part is below 2^(n+1), so 2^(63-n) products stay below 2^64 (the exact bound 2^(64-n) (2^hb - 1)(2^(n-hb) - 1) leaves room for what carry()
+// leaves in the sums); then carry() makes room again: after 2^(62-n) terms for the results' middle polynomial, which takes two products a term, and
+// after twice as many for the others.
 struct Half {
   u32 l, h, s;
 };
@@ -20,16 +21,14 @@ template <bool WIDE>
 struct Reduce {
   u64 q, nq, mh, ml;   // the prime, its negative, floor(2^128 / q)
   u64 w, wp;           // 2^(2 hb) mod q and its companion, at most two units of 2^-64 too small
-  double per_q;        // 2^32 / q
-  float near_q;        // the same, a little too small
+  float near_q;        // 2^32 / q, a little too small
   u32 hb, mask;
   __device__ __forceinline__ explicit Reduce(const DevPrime& P) : q(P.q), nq(0 - P.q), mh(P.prec128_hi), ml(P.prec128_lo) {
     hb = (P.nbits + 1) / 2;
     mask = (1u << hb) - 1;
     w = signed_mod(1ll << (2 * hb), q, mh);
     wp = w * mh + mulhi64(w, ml);
-    per_q = 4294967296.0 / (double)q;
-    near_q = (float)per_q * 0.999999f;
+    near_q = (float)(4294967296.0 / (double)q) * 0.999999f;
   }
 };
 // a * w mod q up to multiples of q: below 5q for any a, with a companion wp of w that is at most two units of 2^-64 too small (the quotient leaves
@@ -45,14 +44,15 @@ struct Acc {
     mm += (u64)x.s * y.s;
     hh += (u64)x.h * y.h;
   }
-  // carries brought up and hh reduced below 3q (2q at primes of over 40 bits): room for as many terms again
+  // carries brought up and hh reduced below 3q (WIDE: the quotient by floor(2^64 / q), below 2^32, of hh's upper word: less than three too small):
+  // room for as many terms again
   template <bool WIDE>
   __device__ __forceinline__ void carry(const Reduce<WIDE>& r) {
     u64 mid = mm - ll - hh + (ll >> r.hb);
     ll = (u32)ll & r.mask;
     hh += mid >> r.hb;
     mid = (u32)mid & r.mask;
-    if (WIDE) hh += (u64)(u32)((double)(u32)(hh >> 32) * r.per_q) * r.nq;
+    if (WIDE) hh += __umulhi((u32)(hh >> 32), (u32)r.mh) * r.nq;
     else      hh -= mulhi64(hh, r.mh) * r.q;
     mm = mid + ll + hh;
   }
@@ -124,6 +124,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linattn_kernel(DevCtx c, Lina
   Acc s[MT][NT][3];
   const u32 period = 1u << min(62 - P.nbits, 24u);
   u32 left = period;  // terms that the sums still take
+  bool second = false;
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -203,9 +204,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linattn_kernel(DevCtx c, Lina
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-              for (int p = 0; p < 3; ++p) s[i][j][p].carry(red);
+            for (int j = 0; j < NT; ++j) {
+              s[i][j][1].carry(red);
+              if (second) s[i][j][0].carry(red), s[i][j][2].carry(red);
+            }
+          second = !second;
           left = period;
         }
         --left;
@@ -305,6 +308,7 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void linattn_shared_kernel
   Acc s[MT][NT][3];
   const u32 period = 1u << min(62 - P.nbits, 24u);
   u32 left = period;  // terms that the sums still take
+  bool second = false;
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -416,9 +420,11 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void linattn_shared_kernel
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-              for (int p = 0; p < 3; ++p) s[i][j][p].carry(red);
+            for (int j = 0; j < NT; ++j) {
+              s[i][j][1].carry(red);
+              if (second) s[i][j][0].carry(red), s[i][j][2].carry(red);
+            }
+          second = !second;
           left = period;
         }
         --left;
