@@ -86,6 +86,7 @@ template <int NP, int MT, int WJ, int WN, bool PACKED>
 __device__ __forceinline__ void linear_tiles(const DevCtx& c, const LinearArgs& a, v4i_t* frag, ulong2* factor, const DevPrime& P, u32 rep, u32 pos, const Columns& cols,
                                              u32 j0) {
   constexpr int G = 4 / WJ;  // column blocks of 16 that a thread stages
+  static_assert(4 % WJ == 0 && WJ * WN % 4 == 0, "all of a step's 256 WN groups of inputs are staged");
   const u32 t = threadIdx.x, lane = t & 63u, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const u32 wj = wave % WJ, wn = wave / WJ;
   const u32 last = (a.n_in - 1) / 64;  // step (n_in > 0)
@@ -397,8 +398,13 @@ static void launch_mfma(const DevCtx& c, const LinearArgs& a, hipStream_t s) {
   u32 tiles = 1;
   while (tiles < 8 && blocks / (2 * tiles) >= 2048) tiles *= 2;
   const dim3 grid((all + tiles - 1) / tiles * j_blocks, a.n_limbs, c.nrep), block(64 * WJ * WN);
-  if (a.packed) hipLaunchKernelGGL((linear_i8_mfma_kernel<MT, WJ, WN, true>), grid, block, 0, s, c, a, j_blocks, log_blocks, tiles);
-  else          hipLaunchKernelGGL((linear_i8_mfma_kernel<MT, WJ, WN, false>), grid, block, 0, s, c, a, j_blocks, log_blocks, tiles);
+  if constexpr (MT * WJ > 2) {  // (linear_pack_outputs)
+    if (a.packed) {
+      hipLaunchKernelGGL((linear_i8_mfma_kernel<MT, WJ, WN, true>), grid, block, 0, s, c, a, j_blocks, log_blocks, tiles);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((linear_i8_mfma_kernel<MT, WJ, WN, false>), grid, block, 0, s, c, a, j_blocks, log_blocks, tiles);
 }
 
 // Outputs whose packed weights fit the workspace at a time (all of them unless the layer is large); 0: the weights are read as they lie
@@ -417,14 +423,14 @@ void launch_linear_i8(const DevCtx& c, const LinearArgs& a, hipStream_t s) {
   if (!linear_fits(c, a)) {
     const u32 n_blocks = (c.N + 255) / 256, j_blocks = (a.n_out + kJ - 1) / kJ;
     hipLaunchKernelGGL(linear_i8_kernel, dim3(n_blocks * j_blocks * a.n_comp * a.rows, a.n_limbs, c.nrep), dim3(256), 0, s, c, a, n_blocks, j_blocks);
-  } else if (a.n_out <= 16) {
-    launch_mfma<1, 1, 4>(c, a, s);
   } else if (a.n_out <= 32) {
-    launch_mfma<2, 1, 4>(c, a, s);
+    launch_mfma<1, 2, 2>(c, a, s);
   } else if (a.n_out <= 64) {
-    launch_mfma<4, 1, 4>(c, a, s);
+    launch_mfma<2, 2, 2>(c, a, s);
   } else if (a.n_out <= 128) {
-    launch_mfma<4, 2, 2>(c, a, s);
+    launch_mfma<2, 4, 1>(c, a, s);
+  } else if (a.n_out <= 192 * ((a.n_out + 255) / 256)) {
+    launch_mfma<3, 4, 1>(c, a, s);
   } else {
     launch_mfma<4, 4, 1>(c, a, s);
   }

@@ -19,10 +19,14 @@ void launch_rope_messages(double* cos_out, double* sin_out, u64 out_stride, cons
   hipLaunchKernelGGL(rope_messages_kernel, dim3((n_pos + 255) / 256, n_pairs), dim3(256), 0, s, cos_out, sin_out, out_stride, pos, pos_stride, n_pos, a);
 }
 
-__global__ __launch_bounds__(256) void rope_kernel(DevCtx c, RopeArgs a, u32 n_blocks) {
+// A lane: one coefficient of a pair, whose table it reads once for up to `per` polynomials (heads and components); `parts` workgroups share a
+// pair's polynomials.
+__global__ __launch_bounds__(256) void rope_kernel(DevCtx c, RopeArgs a, u32 n_blocks, u32 parts, u64 per) {
   u32 b = blockIdx.x;
   const u32 nb = b % n_blocks;
   b /= n_blocks;
+  const u64 first = b % parts * per, end = min(first + per, (u64)a.n_heads * a.n_comp);
+  b /= parts;
   const u32 half = a.dim / 2;
   const u32 i = b % half, row = b / half, rep = c.rep0 + blockIdx.z;
   const u32 pos = a.pos0 + blockIdx.y, gi = limb_prime(pos, a.level, c.L);
@@ -35,24 +39,31 @@ __global__ __launch_bounds__(256) void rope_kernel(DevCtx c, RopeArgs a, u32 n_b
   const u32 f0 = a.interleaved ? 2 * i : i, f1 = a.interleaved ? 2 * i + 1 : i + half;
   const u64* in = reb(c, a.in.d, rep) + row * a.in.row + off;
   u64* out = reb(c, a.out.d, rep) + row * a.out.row + off;
-  for (u32 h = 0; h < a.n_heads; ++h)
-    for (u32 k = 0; k < a.n_comp; ++k) {
-      const u64* p = in + h * a.in.head + k * a.in.comp;
-      u64* y = out + h * a.out.head + k * a.out.comp;
-      const u64 x0 = p[f0 * a.in.col], x1 = p[f1 * a.in.col];
-      U128 s0{0, 0}, s1{0, 0};
-      mac128(s0, x0, C);
-      mac128(s0, x1, nS);
-      mac128(s1, x0, S);
-      mac128(s1, x1, C);
-      y[f0 * a.out.col] = reduce128(s0, P.q, P.prec128_lo, P.prec128_hi);
-      y[f1 * a.out.col] = reduce128(s1, P.q, P.prec128_lo, P.prec128_hi);
-    }
+  u32 h = first / a.n_comp, k = first % a.n_comp;
+  for (u64 p = first; p < end; ++p) {
+    const u64* x = in + h * a.in.head + k * a.in.comp;
+    u64* y = out + h * a.out.head + k * a.out.comp;
+    const u64 x0 = x[f0 * a.in.col], x1 = x[f1 * a.in.col];
+    U128 s0{0, 0}, s1{0, 0};
+    mac128(s0, x0, C);
+    mac128(s0, x1, nS);
+    mac128(s1, x0, S);
+    mac128(s1, x1, C);
+    y[f0 * a.out.col] = reduce128(s0, P.q, P.prec128_lo, P.prec128_hi);
+    y[f1 * a.out.col] = reduce128(s1, P.q, P.prec128_lo, P.prec128_hi);
+    if (++k == a.n_comp) k = 0, ++h;
+  }
 }
 
 void launch_rope(const DevCtx& c, const RopeArgs& a, hipStream_t s) {
   const u32 n_blocks = (c.N + 255) / 256;
-  hipLaunchKernelGGL(rope_kernel, dim3(n_blocks * (a.dim / 2) * a.rows, a.n_limbs, c.nrep), dim3(256), 0, s, c, a, n_blocks);
+  const u64 blocks = (u64)n_blocks * (a.dim / 2) * a.rows, polys = (u64)a.n_heads * a.n_comp;
+  // four workgroups for each of 256 CUs, where there are that many polynomials: 15 heads of 10 at N = 2048 take 8.1 us in place of 22 (one part),
+  // 16 heads of 16 at 8192 29 in place of 34; more parts than that read the tables again for nothing
+  u32 parts = 1;
+  while (parts < polys && blocks * a.n_limbs * c.nrep * parts < 1024) parts *= 2;
+  const u64 per = (polys + parts - 1) / parts;
+  hipLaunchKernelGGL(rope_kernel, dim3(blocks * parts, a.n_limbs, c.nrep), dim3(256), 0, s, c, a, n_blocks, parts, per);
 }
 
 }  // namespace acehip

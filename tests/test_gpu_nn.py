@@ -143,7 +143,7 @@ def test_linear_shapes(contexts, name, level, limbs, n_in, n_out):
     linear_case(rt, level, limbs, 1, n_in, n_out, 2)
 
 
-@pytest.mark.parametrize("n_in,n_out", [(1, 300), (300, 1), (257, 129), (63, 257), (128, 128), (192, 65)])
+@pytest.mark.parametrize("n_in,n_out", [(1, 300), (300, 1), (257, 129), (63, 257), (128, 128), (192, 65), (65, 200), (70, 32), (64, 385)])
 @pytest.mark.parametrize("mul,tok", [(True, False), (False, True), (True, True)])
 def test_linear_tiles_and_scales(contexts, n_in, n_out, mul, tok):
     linear_case(contexts("n64"), 2, [0, 1], 2, n_in, n_out, 1, mul, tok)
@@ -194,7 +194,7 @@ def mul_mod(a, b, q):
     return np.where(r >= q, r - q, r).astype(np.uint64)
 
 
-@pytest.mark.parametrize("n_in,n_out,rows,n_comp", [(65, 257, 1, 2), (40, 300, 1, 2), (129, 144, 3, 1), (192, 260, 1, 3), (3, 33, 5, 3)])
+@pytest.mark.parametrize("n_in,n_out,rows,n_comp", [(65, 257, 1, 2), (40, 300, 1, 2), (129, 144, 3, 1), (192, 260, 1, 3), (3, 33, 5, 3), (65, 250, 1, 2), (40, 96, 2, 2), (70, 20, 3, 2)])
 def test_linear_many_column_blocks(contexts, n_in, n_out, rows, n_comp):
     """large enough a ring that a workgroup takes several column blocks, across polynomials and rows"""
     rt = _open.setdefault("n16384", A.AceHip(16384, 2, 60, 50, 1))
@@ -272,7 +272,7 @@ def rope_case(rt, level, limbs, heads, rows, dim, n_comp, interleaved=False, ord
 
 
 @pytest.mark.parametrize("name,level,limbs", [("n16", 4, [0, 1, 2, 3]), ("n16", 3, [2, 3, 4]), ("n32", 3, [0, 1, 2, 3]), ("n64", 3, [1, 2]), ("n1024", 2, [0, 1, 2]), ("n2048", 1, [0])])
-@pytest.mark.parametrize("heads,rows,dim,n_comp", [(1, 1, 2, 1), (2, 3, 6, 2), (5, 1, 10, 2), (3, 2, 4, 3)])
+@pytest.mark.parametrize("heads,rows,dim,n_comp", [(1, 1, 2, 1), (2, 3, 6, 2), (5, 1, 10, 2), (3, 2, 4, 3), (11, 1, 2, 2)])
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_rope(contexts, name, level, limbs, heads, rows, dim, n_comp, interleaved):
     rope_case(contexts(name), level, limbs, heads, rows, dim, n_comp, interleaved)
@@ -292,6 +292,30 @@ def test_rope_extremes(contexts, name, kind):
 
 
 # ---- linear attention ------------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dim", [12, 6, 2])
+def test_rope_in_large_launches(dim):
+    """a ring of 16384: one workgroup for all heads of a pair, or several"""
+    rt = _open.setdefault("n16384", A.AceHip(16384, 2, 60, 50, 1))
+    heads, comps, N = 3, 2, rt.N
+    q = np.array([rt.primes[i] for i in range(3)], dtype=np.uint64)[:, None]
+    rng = np.random.default_rng(dim)
+    draw = lambda *shape: np.stack([rng.integers(0, p[0], size=(*shape, N), dtype=np.uint64) for p in q], axis=-2)
+    x, c, s = draw(heads, dim, comps), draw(dim // 2, 1), draw(dim // 2, 1)
+    dx, dc, ds, dy = (dev(rt, v) for v in (x, c, s, np.full_like(x, 7)))
+    strides = dict(head=dim * comps * 3 * N, col=comps * 3 * N, comp=3 * N)
+    rt.rope(rt.mat(dy.ptr, **strides), rt.mat(dx.ptr, **strides), dc.ptr, ds.ptr, 3 * N, 0, heads, 1, dim, comps, 2, n_limbs=3)
+    x0, x1 = x[:, :dim // 2], x[:, dim // 2:]
+    full = lambda v: np.broadcast_to(v, x0.shape)
+    y0 = (mul_mod(x0, full(c), q) + q - mul_mod(x1, full(s), q)) % q
+    y1 = (mul_mod(x0, full(s), q) + mul_mod(x1, full(c), q)) % q
+    assert np.array_equal(dy.download(x.shape), np.concatenate([y0, y1], axis=1))
+    for d in (dx, dc, ds, dy):
+        d.free()
+
+
+# ---- linear attention ------------------------------------------------------------------------------------------------------------------
 def pair(a, b):
     """product of two ciphertexts [2][limb][N] before relinearisation"""
     return np.stack([a[0] * b[0], a[0] * b[1] + a[1] * b[0], a[1] * b[1]])
@@ -306,13 +330,16 @@ def factors(rng, *shape):
 class Attn:
     """operands of the three calls for one set of sizes"""
 
+    Block = Block
+
     def __init__(self, rt, level, limbs, H, kv, nq, nk, dk, dv, orders=("hrcp",) * 6, pad=0, kind=None, seed=5, factor=True):
         self.rt, self.level, self.limbs, self.sizes = rt, level, limbs, (H, kv, nq, nk, dk, dv)
+        self.n = rt.N
         rng = np.random.default_rng(seed)
         b = iter(range(100))
 
         def block(*shape, order):
-            return Block(rt, shape, level, limbs, order, pad, seed=seed + next(b), data=extreme(rt, shape, level, limbs, kind) if kind else None)
+            return self.Block(rt, shape, level, limbs, order, pad, seed=seed + next(b), data=extreme(rt, shape, level, limbs, kind) if kind else None)
 
         self.q = block(H, nq, dk, 2, order=orders[0])
         self.k = block(kv, nk, dk, 2, order=orders[1])
@@ -327,7 +354,7 @@ class Attn:
         self.dd = [dev(rt, f) if f.size else None for f in (self.din, self.dec, self.keep)]
 
     def result(self, *shape):
-        return Block(self.rt, (*shape, 3), self.level, self.limbs, self.order, self.pad, data=False)
+        return self.Block(self.rt, (*shape, 3), self.level, self.limbs, self.order, self.pad, data=False)
 
     def range(self):
         return dict(pos0=self.limbs[0], n_limbs=len(self.limbs))
@@ -340,7 +367,7 @@ class Attn:
         y = self.result(H, nq, nk)
         self.rt.linattn_scores(y.mat, self.q.mat, self.k.mat, H, kv, nq, nk, dk, self.level, causal=causal, **self.range())
         q, k = self.q.values(), self.k.values()
-        want = np.zeros((H, nq, nk, 3, len(self.limbs), self.rt.N), dtype=object)
+        want = np.zeros((H, nq, nk, 3, len(self.limbs), self.n), dtype=object)
         for h, t, s in itertools.product(range(H), range(nq), range(nk)):
             want[h, t, s] = sum((pair(q[h, t, a], k[h * kv // H, s, a]) for a in range(dk)), want[h, t, s]) % y.q()
         y.check(want, (lambda ix: ix[2] <= ix[1] + nk - nq) if causal else None)
@@ -353,7 +380,7 @@ class Attn:
         self.rt.linattn_out(y.mat, self.q.mat if state else None, self.S.mat if state else None, self.p.mat if chunk else None, self.v.mat if chunk else None, H, kv, nq, nk,
                             dk, dv, self.level, d_in=self.ptr(0, factor), d_decay=self.ptr(1, dec), causal=causal, **self.range())
         q, S, p, v = self.q.values(), self.S.values(), self.p.values(), self.v.values()
-        want = np.zeros((H, nq, dv, 3, len(self.limbs), self.rt.N), dtype=object)
+        want = np.zeros((H, nq, dv, 3, len(self.limbs), self.n), dtype=object)
         for h, t, b in itertools.product(range(H), range(nq), range(dv)):
             r = want[h, t, b]
             if state:
@@ -372,13 +399,13 @@ class Attn:
         y = self.result(H, dk, dv)
         S = self.S
         if in_place:
-            S = Block(self.rt, (H, dk, dv, 3), self.level, self.limbs, self.order, self.pad, seed=99)
+            S = self.Block(self.rt, (H, dk, dv, 3), self.level, self.limbs, self.order, self.pad, seed=99)
             y.free()
             y = S
         self.rt.linattn_state(y.mat, S.mat if kept else None, self.k.mat, self.v.mat, H, kv, nk, dk, dv, self.level, d_keep=self.ptr(2, factor), d_decay=self.ptr(1, factor),
                               **self.range())
         Sv, k, v = S.values(), self.k.values(), self.v.values()
-        want = np.zeros((H, dk, dv, 3, len(self.limbs), self.rt.N), dtype=object)
+        want = np.zeros((H, dk, dv, 3, len(self.limbs), self.n), dtype=object)
         for h, a, b in itertools.product(range(H), range(dk), range(dv)):
             r = want[h, a, b].copy()
             for s in range(nk):
@@ -439,6 +466,51 @@ def test_linear_attention_extremes(contexts, name, kind, factor):
     a.scores()
     a.out(factor=factor)
     a.state(factor=factor)
+    a.free()
+
+
+class Sampled(Block):
+    """of a large ring, compared at some coefficients"""
+
+    AT = np.array([0, 1, 62, 63, 64, 255, 256, 4097, 9999, 16382, 16383])
+
+    def values(self):
+        got = np.zeros((*self.shape, len(self.limbs), len(self.AT)), dtype=object)
+        for ix, k, w in self.spots(self.host):
+            got[ix][k] = w[self.AT].astype(object)
+        return got
+
+    def check(self, want, written=None):
+        got = self.buf.download()
+        for (ix, k, w), (_, _, before) in zip(self.spots(got), self.spots(self.host)):
+            if written is None or written(ix):
+                assert np.array_equal(w[self.AT], want[ix][k].astype(np.uint64)), (ix, k)
+                w[:] = before
+        assert np.array_equal(got, self.host)
+
+
+class LargeAttn(Attn):
+    Block = Sampled
+
+    def __init__(self, *args, **kw):
+        super().__init__(*args, **kw)
+        self.n = len(Sampled.AT)
+
+
+@pytest.mark.parametrize("sizes,kind", [((2, 1, 1, 1, 5, 18), None), ((2, 1, 3, 4, 3, 9), None), ((2, 1, 9, 9, 10, 6), None), ((1, 1, 5, 66, 2, 5), None), ((1, 1, 6, 17, 33, 5), "top"),
+                                        ((1, 1, 1, 20, 33, 17), "top"), ((1, 1, 4, 9, 20, 4), "alternate")], ids=str)
+def test_linear_attention_in_large_launches(sizes, kind):
+    """a launch that fills the card (a ring of 16384): rows, small and large sets of results, sums over many terms"""
+    rt = _open.setdefault("n16384", A.AceHip(16384, 2, 60, 50, 1))
+    a = LargeAttn(rt, 2, [0, 1, 2], *sizes, kind=kind)
+    a.scores()
+    a.scores(causal=False)
+    a.out()
+    a.out(causal=False)
+    a.out(state=False, factor=False)
+    a.state()
+    a.state(factor=False)
+    a.state(in_place=True)
     a.free()
 
 
