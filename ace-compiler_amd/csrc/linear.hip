@@ -341,8 +341,8 @@ __global__ __launch_bounds__(64 * WJ * WN, 2) void linear_i8_mfma_kernel(DevCtx 
   else                linear_tiles<8, MT, WJ, WN, PACKED>(c, a, frag, factor, P, rep, pos, cols, j0);
 }
 
-// What the matrix-core form does not take (linear_fits: rings below 64, primes below 2^40, strides of over 32 MiB): one coefficient per lane, kJ outputs: residues split at 31 bits, so that each half times a weight is one multiply-add into a
-// signed 64-bit sum (|sum| <= 2^31 * 2^7 * 2^16 inputs).
+// What the matrix-core form does not take (linear_fits: rings below 64, primes below 2^40, inputs that share words or lie over 32 MiB apart): one
+// coefficient per lane, kJ outputs, residues split at 31 bits, so that each half times a weight is one multiply-add into a signed 64-bit sum (|sum| <= 2^31 * 2^7 * 2^16 inputs).
 constexpr u32 kJ = 8;
 __global__ __launch_bounds__(256) void linear_i8_kernel(DevCtx c, LinearArgs a, u32 n_blocks, u32 j_blocks) {
   u32 b = blockIdx.x;
@@ -382,9 +382,10 @@ __global__ __launch_bounds__(256) void linear_i8_kernel(DevCtx c, LinearArgs a, 
   }
 }
 
-// the matrix-core form: rings and primes that it takes, lane offsets below 2^32, and an array of weights that holds a fragment of 16 bytes
+// the matrix-core form: rings and primes that it takes, inputs that lie apart (a descriptor that ends behind the last one reads zeros for those past
+// it), lane offsets below 2^32, and an array of weights that holds a fragment of 16 bytes
 static bool linear_fits(const DevCtx& c, const LinearArgs& a) {
-  return c.N >= 64 && a.wide_primes && a.in.col <= (1u << 22) && a.out.col <= (1u << 23) && a.ld_w <= (1u << 24) && a.n_in != 0 &&
+  return c.N >= 64 && a.wide_primes && a.in.col >= c.N && a.in.col <= (1u << 22) && a.out.col <= (1u << 23) && a.ld_w <= (1u << 24) && a.n_in != 0 &&
          (u64)(a.n_out - 1) * a.ld_w + a.n_in >= 16;
 }
 

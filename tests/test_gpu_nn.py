@@ -225,6 +225,26 @@ def test_linear_many_column_blocks(contexts, n_in, n_out, rows, n_comp):
         d.free()
 
 
+@pytest.mark.parametrize("same", ["row", "col", "comp", "all"])
+@pytest.mark.parametrize("n_in,n_out", [(5, 3), (70, 40)])
+def test_linear_shared_inputs(contexts, same, n_in, n_out):
+    """strides of zero: one row, one input or one polynomial for all"""
+    rt = contexts("n64")
+    level, limbs, rows, comps = 3, [0, 1, 2], 2, 2
+    shape = dict(row=rows, col=n_in, comp=comps)
+    shape = {k: 1 if same in (k, "all") else n for k, n in shape.items()}
+    x = Block(rt, (1, *shape.values()), level, limbs)
+    strides = {k: 0 if shape[k] == 1 else s for k, s in zip(shape, x.strides[1:])}
+    y = Block(rt, (1, rows, n_out, comps), level, limbs, data=False)
+    w = np.random.default_rng(8).integers(-128, 128, size=(n_out, n_in)).astype(np.int8)
+    dw = dev(rt, w)
+    rt.linear_i8(y.mat, rt.mat(x.buf.ptr, **strides), dw.ptr, n_in, rows, n_in, n_out, comps, level)
+    v = np.broadcast_to(x.values()[0], (rows, n_in, comps, len(limbs), rt.N))
+    y.check(np.tensordot(w.astype(object), v, (1, 1)).swapaxes(0, 1)[None] % y.q())
+    for b in (x, y, dw):
+        b.free()
+
+
 def test_linear_empty_sum_is_zero(contexts):
     linear_case(contexts("n64"), 2, [0, 1], 1, 0, 5, 2, True, True)
 
@@ -289,9 +309,6 @@ def test_rope_layouts(contexts, order, pad, in_place, shared_rows):
 @pytest.mark.parametrize("kind", ["top", "alternate"])
 def test_rope_extremes(contexts, name, kind):
     rope_case(contexts(name), 2, [0, 1, 2], 1, 1, 4, 2, kind=kind)
-
-
-# ---- linear attention ------------------------------------------------------------------------------------------------------------------
 
 
 @pytest.mark.parametrize("dim", [12, 6, 2])
