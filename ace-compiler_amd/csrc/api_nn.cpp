@@ -256,9 +256,9 @@ int acehip_rope(acehip_ctx* c, const acehip_mat* out, const acehip_mat* in, cons
 }
 
 // the counts of a linear attention call that its entry points share
-static int check_heads(const Call& k, u32 n_heads, u32 n_kv_heads, u32 n_q, u32 n_k) {
+static int check_heads(const Call& k, u32 n_heads, u32 n_kv_heads, u32 n_q, u32 n_k, u32 dim) {
   if (n_heads && (n_kv_heads == 0 || n_heads % n_kv_heads)) return k.bad("n_heads is not a multiple of n_kv_heads");
-  if ((n_q | n_k) >> 31) return k.bad("2^31 or more tokens");
+  if ((n_q | n_k | dim) >> 31) return k.bad("2^31 or more tokens or features");
   return ACEHIP_OK;
 }
 // pairs (query, key) of a call: of a causal one, the last query sees all keys, each one before it one key less
@@ -282,7 +282,7 @@ int acehip_linattn_scores(acehip_ctx* c, const acehip_mat* p3, const acehip_mat*
                           uint32_t n_k, uint32_t dim, int causal, uint32_t level, uint32_t pos0, uint32_t n_limbs, acehip_stream s) {
   const Call k{c, "acehip_linattn_scores", level, pos0, n_limbs};
   if (int e = k.range()) return e;
-  if (int e = check_heads(k, n_heads, n_kv_heads, n_q, n_k)) return e;
+  if (int e = check_heads(k, n_heads, n_kv_heads, n_q, n_k, dim)) return e;
   View y, vq, vk;
   if (int e = k.view(y, p3, n_heads, n_q, n_k, 3)) return e;
   if (y.empty()) return check_dev(c);
@@ -307,7 +307,7 @@ int acehip_linattn_out(acehip_ctx* c, const acehip_mat* o3, const acehip_mat* q,
                        const int64_t* d_decay, int causal, uint32_t level, uint32_t pos0, uint32_t n_limbs, acehip_stream s) {
   const Call k{c, "acehip_linattn_out", level, pos0, n_limbs};
   if (int e = k.range()) return e;
-  if (int e = check_heads(k, n_heads, n_kv_heads, n_q, n_k)) return e;
+  if (int e = check_heads(k, n_heads, n_kv_heads, n_q, n_k, dim_k)) return e;
   if (!p != !v) return k.bad("scores and values come together");
   if (!q != !state) return k.bad("queries and state come together");
   View y, vq, vs, vp, vv;
@@ -355,7 +355,7 @@ int acehip_linattn_state(acehip_ctx* c, const acehip_mat* s3, const acehip_mat* 
                          uint32_t pos0, uint32_t n_limbs, acehip_stream s) {
   const Call k{c, "acehip_linattn_state", level, pos0, n_limbs};
   if (int e = k.range()) return e;
-  if (int e = check_heads(k, n_heads, n_kv_heads, 1, n_k)) return e;
+  if (int e = check_heads(k, n_heads, n_kv_heads, 1, n_k, dim_k)) return e;
   View y, vs, vk, vv;
   if (int e = k.view(y, s3, n_heads, dim_k, dim_v, 3)) return e;
   if (y.empty()) return check_dev(c);

@@ -363,7 +363,9 @@ typedef struct acehip_mat {
 /* Linear layer with int8 weights, a factor for each output channel and a plaintext for each row of tokens:
  *   out[r][j] = tok[r] (*) mul[j] * sum_{i < n_in} w[j][i] in[r][i]      for each of the n_comp polynomials of the ciphertexts
  * in: rows x n_in, out: rows x n_out (head_stride unused).  d_w: [n_out][ld_w] bytes, ld_w >= n_in, no alignment asked.  d_mul: [n_out] or NULL.
- * d_tok: plaintext polynomial of row r (encoded scales of its tokens: 0 / 1 masks padding) at d_tok + r*tok_stride, or NULL. */
+ * d_tok: plaintext polynomial of row r (encoded scales of its tokens: 0 / 1 masks padding) at d_tok + r*tok_stride, or NULL.
+ * The weights of more than 32 outputs are laid out in the context's workspace on `stream`: like the pipelines that keep scratch there, calls on
+ * one context follow each other, on one stream or ordered between streams, and graphs captured from them are not replayed at the same time. */
 #define ACEHIP_LINEAR_MAX_IN 65536
 int acehip_linear_i8(acehip_ctx* ctx, const acehip_mat* out, const acehip_mat* in, const int8_t* d_w, size_t ld_w, uint32_t rows, uint32_t n_in,
                      uint32_t n_out, uint32_t n_comp, const int64_t* d_mul, const uint64_t* d_tok, size_t tok_stride, uint32_t level, uint32_t pos0,
@@ -386,6 +388,7 @@ int acehip_rope(acehip_ctx* ctx, const acehip_mat* out, const acehip_mat* in, co
 /* Linear attention with a decay for each head.  (x) is the product of two ciphertexts before relinearisation, (a0, a1) (x) (b0, b1) =
  * (a0 b0, a0 b1 + a1 b0, a1 b1): operands have two polynomials, results three.  Head h reads the keys and values of head
  * h' = h / (n_heads / n_kv_heads).  Rows of q, key, v are tokens, columns features.
+ * Counts of tokens and features are below 2^31.
  * A chunk of a prompt: scores (relinearise, rescale), out with the state so far, state.  One token (recurrent form): state with n_k = 1
  * (relinearise, rescale), then out with n_q = 1 and no scores.
  *

@@ -218,6 +218,10 @@ def test_linear_attention(rt):
     for cls in (Scores, Out, State):
         for bad in (dict(kv=3), dict(kv=0), dict(kv=8), dict(nk=1 << 31)):
             assert changed(cls, **bad).call(rt) == EINVAL, bad
+    one = A.binding.Mat(BASE + FAR, 0, 0, 0, 0)  # (strides of zero: any count of features lies in memory)
+    assert changed(Scores, dim=1 << 31, q=one, k=one).call(rt) == EINVAL
+    assert changed(Scores, dim=(1 << 31) - 1, q=one, k=one).call(rt) == ENODEV
+    assert changed(Out, dk=1 << 31, q=one, S=one).call(rt) == EINVAL
     for bad in (dict(q=None), dict(S=None), dict(p=None), dict(v=None), dict(causal=0), dict(din=BASE + 5 * FAR + 4), dict(decay=BASE + 8)):
         assert changed(Out, **bad).call(rt) == EINVAL, bad
     for good in (dict(q=None, S=None), dict(p=None, v=None), dict(q=None, S=None, p=None, v=None), dict(causal=0, decay=None), dict(nk=0), dict(dk=0), dict(nq=0),
