@@ -28,7 +28,7 @@ struct Reduce {
     mask = (1u << hb) - 1;
     w = signed_mod(1ll << (2 * hb), q, mh);
     wp = w * mh + mulhi64(w, ml);
-    near_q = (float)(4294967296.0 / (double)q) * 0.999999f;
+    near_q = __builtin_fmaf((float)(u32)(ml >> 32), 0x1p-32f, (float)mh) * (0x1p-32f * 0.999999f);
   }
 };
 // a * w mod q up to multiples of q: below 5q for any a, with a companion wp of w that is at most two units of 2^-64 too small (the quotient leaves
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linattn_kernel(DevCtx c, Lina
   }
   t = __builtin_amdgcn_readfirstlane(t);
   g = __builtin_amdgcn_readfirstlane(g);
-  const u32 nb = g % n_blocks, h = g / n_blocks, rep = c.rep0 + blockIdx.z;
+  const u32 nb = g & (n_blocks - 1), h = g >> __builtin_ctz(n_blocks), rep = c.rep0 + blockIdx.z;
   const u32 lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const u32 wg_m = (t / n_tiles) * (MT * WM), m0 = wg_m + (wave / WN) * MT, j0 = ((t % n_tiles) * WN + wave % WN) * NT;
   const u32 pos = a.pos0 + blockIdx.y, gi = limb_prime(pos, a.level, c.L);
@@ -152,8 +152,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linattn_kernel(DevCtx c, Lina
     // a causal sum ends with the last key that a row of the wave (of the workgroup: the factors) sees
     const u32 K = causal ? (u32)min((int64_t)t.K, max(last + 1, (int64_t)0)) : t.K, K_wg = causal ? (u32)min((int64_t)t.K, max(wg_last + 1, (int64_t)0)) : t.K;
     if (K_wg == 0) continue;
-    const u64* A = reb(c, t.a.d, rep) + (h / t.a_group) * t.a.head + limb;
-    const u64* B = reb(c, t.b.d, rep) + (h / t.b_group) * t.b.head + limb;
+    const u64* A = reb(c, t.a.d, rep) + (t.a_group == 1 ? h : h / t.a_group) * t.a.head + limb;
+    const u64* B = reb(c, t.b.d, rep) + (t.b_group == 1 ? h : h / t.b_group) * t.b.head + limb;
     const u64 a_col = t.a.col, b_row = t.b.row;
     const u64 *pa[MT][2], *pb[NT][2];  // where the next term's residues lie
 #pragma unroll
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void linattn_shared_kernel
   }
   t = __builtin_amdgcn_readfirstlane(t);
   g = __builtin_amdgcn_readfirstlane(g);
-  const u32 nb = g % n_blocks, h = g / n_blocks, rep = c.rep0 + blockIdx.z;
+  const u32 nb = g & (n_blocks - 1), h = g >> __builtin_ctz(n_blocks), rep = c.rep0 + blockIdx.z;
   const u32 lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const u32 wg_m = (t / n_tiles) * M, wg_j = (t % n_tiles) * N;
   const u32 wm = (wave / WN) * MT, wn = (wave % WN) * NT, m0 = wg_m + wm, j0 = wg_j + wn;
@@ -303,7 +303,11 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void linattn_shared_kernel
   const u32 hb = red.hb;
   const u32 n = nb * 64 + lane, at = 8 * n;
   const u64 limb = (u64)pos * c.N;
-  auto read = [&](const u64* p) { return *(const GLOBAL u64*)(uniform(p) + at); };
+  auto read = [&](const u64* p) {
+    u32 o = at;
+    asm("" : "+v"(o));  // (opaque: a load takes the uniform base and 32-bit offset as they are)
+    return *(const GLOBAL u64*)(uniform(p) + o);
+  };
 
   Acc s[MT][NT][3];
   const u32 period = 1u << min(62 - P.nbits, 24u);
@@ -335,8 +339,8 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void linattn_shared_kernel
     const u32 K = causal ? (u32)min((int64_t)t.K, max(wg_last + 1, (int64_t)0)) : t.K;  // of the workgroup; K_own: of this wave's results
     const u32 K_own = idle ? 0 : causal ? (u32)min((int64_t)t.K, max(last + 1, (int64_t)0)) : t.K;
     if (K == 0) continue;
-    const u64* A = reb(c, t.a.d, rep) + (h / t.a_group) * t.a.head + limb;
-    const u64* B = reb(c, t.b.d, rep) + (h / t.b_group) * t.b.head + limb;
+    const u64* A = reb(c, t.a.d, rep) + (t.a_group == 1 ? h : h / t.a_group) * t.a.head + limb;
+    const u64* B = reb(c, t.b.d, rep) + (t.b_group == 1 ? h : h / t.b_group) * t.b.head + limb;
     // the wave's share: row wave + r*W of the tile's rows, then columns
     const u64* from[R][2];
     u64 next[R];
