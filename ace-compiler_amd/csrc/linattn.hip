@@ -479,14 +479,13 @@ static void launch_shared(const DevCtx& c, const LinattnArgs& a, hipStream_t s) 
 }
 
 void launch_linattn(const DevCtx& c, const LinattnArgs& a, hipStream_t s) {
-  const bool row = a.M == 1, shared = a.M > 4 && a.Nn > 4 && a.t1.K + a.t2.K >= 8;
-  const u32 m = row ? 1 : 4, n = row ? 16 : shared ? 4 : 8;  // results of a workgroup below
+  const bool row = a.M == 1;
+  const u32 m = row ? 1 : 4, n = row ? 16 : 4;  // results of a workgroup below
   const u64 groups = (u64)((c.N + 63) / 64) * ((a.M + m - 1) / m) * ((a.Nn + n - 1) / n) * a.n_heads * a.n_limbs * c.nrep;
-  if (!a.wide_primes)                    launch_tiles<1, 1, 1, 1, false>(c, a, s);
-  else if (c.N >= 64 && groups < 512)    launch_shared<1, 1, 2, 2, 2, 4>(c, a, s);
-  else if (row)                          launch_tiles<1, 4, 1, 4, true>(c, a, s);
-  else if (c.N >= 64 && shared)          launch_shared<2, 2, 2, 2, 1, 4>(c, a, s);
-  else                                   launch_tiles<2, 4, 2, 2, true>(c, a, s);
+  if (!a.wide_primes)                 launch_tiles<1, 1, 1, 1, false>(c, a, s);
+  else if (c.N >= 64 && groups < 512) launch_shared<1, 1, 2, 2, 2, 4>(c, a, s);
+  else if (c.N >= 64 && !row)         launch_shared<2, 2, 2, 2, 1, 4>(c, a, s);
+  else                                launch_tiles<1, 4, 1, 4, true>(c, a, s);
 }
 
 }  // namespace acehip
