@@ -81,6 +81,8 @@ __device__ __forceinline__ const GLOBAL char* uniform(const u64* p) {
 // A wave: 64 coefficients, MT x NT results (3 sums of 3 words each); a workgroup: WM x WN such tiles of the same coefficients, whose operands
 // meet in the CU's L1.  Per term of the sums a lane reads 2 (MT + NT) residues and makes 12 MT NT multiply-adds.
 // WIDE: primes above 2^32 (the reduction's quotient from three partial products).
+// In use for one row of results, where nothing but the row is read twice: bound by memory (32 x 32 states read by one token, two heads and limbs at N = 1024,
+// 10 us from the caches; 48 x 48, four heads, three limbs at 8192: 3.8 GB in 0.72 ms, 5.3 TB/s), and for the chains and rings that the form below does not take.
 template <int MT, int NT, int WM, int WN, bool WIDE>
 __global__ __launch_bounds__(64 * WM * WN, 2) void linattn_kernel(DevCtx c, LinattnArgs a, u32 n_blocks, u32 m_tiles, u32 n_tiles) {
   constexpr u32 KC = 64;  // terms whose factors are prepared at a time
@@ -259,8 +261,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linattn_kernel(DevCtx c, Lina
         for (int p = 0; p < 3; ++p) *(GLOBAL u64*)((GLOBAL char*)uniform(y + row[i] * a.out.row + col[j] * a.out.col + p * a.out.comp) + at) = s[i][j][p].value(red);
 }
 
-// The same for larger products, with the operands of a workgroup's waves shared through LDS: every row of A and column of B is read by one wave,
-// has its factor and mask applied and its residues split in halves there, KS terms at a time and one stage ahead.
+// The same with the operands of a workgroup's waves shared through LDS: every row of A and column of B is read by one wave, has its factor and mask
+// applied and its residues split in halves there, KS terms at a time and one stage ahead.
+// Bound by the integer instructions: 106 for a wave's term of 4 x 64 results (48 multiply-adds, 11 to add halves and read LDS, 15 staging, up to 40 of
+// carries at primes of 60 bits, the rest start and end of a sum of 32 terms), all at about four cycles.  32 x 32 causal scores of 32 features, four heads
+// of two, three limbs at N = 4096: 1.01 ms, 10^10 multiply-adds (30 % of the rate they reach alone), 1.8 GB.  One token into 32 x 32 states, four
+// heads and limbs at 8192: 1.27 ms for 5.5 GB (4.3 TB/s), bound by memory.
+// Sums of int8 products on the matrix cores, as in linear.hip, cost as many instructions: tiles of 16 x 16 leave a byte 16 uses for its transposition,
+// and the reductions at the end weigh more at sums this short; that form took 1.63 ms.
+// Tiles of 2 x 2 results in 2 x 2 waves: 2 x 4 results (half the waves) 1.56 ms, 2 x 4 waves 1.52, two terms a stage 1.16.
 __device__ __forceinline__ void lds_barrier() {  // LDS writes are visible, requests to memory stay in flight
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
   __builtin_amdgcn_s_barrier();
@@ -478,6 +487,10 @@ static void launch_shared(const DevCtx& c, const LinattnArgs& a, hipStream_t s) 
                      a, n_blocks, m_tiles, n_tiles);
 }
 
+// One row: its operands are read once whatever the form, and waiting for each other costs (48 x 48 state at N = 8192: 0.72 ms, 0.86 shared).  Two rows or
+// more share (2 x 40 x 4 scores at 8192: 53 us, 91 by linattn_kernel's tiles of 4 x 8; 64 x 2 state of four tokens 0.55 ms, 1.09).  Launches that leave
+// half the places for workgroups empty take one result a wave and two terms a stage (9 x 9 scores of 51 features at 2048: 25 us, 38 by 2 x 2; a 32 x 32
+// state read by one token at 1024, two heads and limbs, 18.5 us, 22.6 by rows; from 512 workgroups on it loses: 8 x 8 scores of 24 features at 4096: 27 us, 24).
 void launch_linattn(const DevCtx& c, const LinattnArgs& a, hipStream_t s) {
   const bool row = a.M == 1;
   const u32 m = row ? 1 : 4, n = row ? 16 : 4;  // results of a workgroup below

@@ -11,10 +11,14 @@ namespace acehip {
 // NP signed bytes d_p (x = sum d_p 256^p: the bytes of (x + C) ^ C, C = 0x80 in every byte), so
 //   sum_i w_ji x_i = sum_p 256^p (W D_p)_j ,
 // NP int8 matrix products with exact 32-bit sums (|sum| <= 2^14 * 2^16 inputs), joined in 64-bit parts and reduced once.
-// Layout: a workgroup of four waves takes 16 WN columns and 16 MT WJ outputs, WJ waves along the outputs and WN = 4 / WJ along the columns.  A step
-// is 64 inputs: the residues are read once by the workgroup, their bytes transposed in registers (four inputs of a column by v_perm_b32) and left in
-// LDS as the B fragments of v_mfma_i32_16x16x64_i8 (1 KiB each, read without bank conflicts); the weights' rows are the A fragments as they lie
-// in memory.  Residues are requested two steps ahead, weights one.
+// Layout: a workgroup of four waves takes 16 WN columns and 16 MT WJ outputs, WJ waves along the outputs and WN along the columns.  A step is 64
+// inputs: the residues are read once by the workgroup, their bytes transposed in registers (four inputs of a column by v_perm_b32) and left in LDS
+// as the B fragments of v_mfma_i32_16x16x64_i8 (1 KiB each, read without bank conflicts); the weights are the A fragments, packed by a kernel of
+// their own (or, up to 32 outputs, as their rows lie in memory).  Residues are requested three steps ahead and staged one ahead, weights one.
+// Bound: up to 128 outputs by memory (800 -> 32, N = 16384, two rows, three limbs: 0.28 ms, 4.7 TB/s; 333 -> 77, N = 4096, three rows: 59 us, 4.1 TB/s);
+// above by the matrix cores and the power that they draw (768 -> 2304 at N = 16384: 1.64 ms, 2.78 * 10^15 int8 operations, 1.70 POP/s; the product
+// with its LDS reads and stores alone takes 0.92 ms, staging 0.15, the loads 0.4 and the reduction 0.2: the parts add up since the clock falls to
+// 1.96 GHz; a library's int8 product of 8192^3 reaches 2.08 POP/s on this card).
 // ------------------------------------------------------------------------------------------------
 typedef int v4i_t __attribute__((ext_vector_type(4)));
 typedef int v4i_any_t __attribute__((ext_vector_type(4), aligned(1)));
@@ -48,7 +52,9 @@ __device__ __forceinline__ void lds_barrier() {
 }
 
 // Weights as A fragments, [tile of 16 outputs][step][lane] of 16 bytes, zero past the matrix.  In memory a fragment's lanes read 16 bytes from each of
-// 16 rows, which costs the L1 cache 64 look-ups (four waves a fragment long: the product waits for them); packed, a fragment is 1 KiB in a row.
+// 16 rows, which costs the L1 cache 64 look-ups (four waves a fragment long: the product waits for them); packed, a fragment is 1 KiB in a row:
+// 2.62 -> 1.91 ms (768 -> 2304 at N = 16384), with the launch.  Up to 32 outputs one wave reads each fragment and the launch costs what it saves
+// (333 -> 30, three rows at 2048: 19.6 us unpacked, 20.3 packed; one row at 1024: 8.9 and 11.6; 800 -> 32 at 16384: 276 and 268).
 __global__ __launch_bounds__(256) void linear_pack_kernel(const int8_t* w, u64 ld_w, u32 n_in, u32 n_out, u32 steps, u32 n_frags, v4i_t* out) {
   const u32 f = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63u;
   if (f >= n_frags) return;
@@ -394,10 +400,12 @@ static void launch_mfma(const DevCtx& c, const LinearArgs& a, hipStream_t s) {
   u32 log_blocks = 0;
   while ((16u * WN << log_blocks) < c.N) ++log_blocks;
   const u32 all = (a.rows * a.n_comp) << log_blocks, j_blocks = (a.n_out + 16 * MT * WJ - 1) / (16 * MT * WJ);
-  // several column blocks to a workgroup once the card is filled a few times over (two workgroups on each of 256 CUs)
+  // several column blocks to a workgroup while two for each place are left (two workgroups on each of 256 CUs): one block each takes 1.81 ms in place
+  // of 1.64 (768 -> 2304 at N = 16384, three limbs), 235 us in place of 206 (512 -> 512 at 8192, four limbs); fewer workgroups leave places empty at
+  // the end (77 outputs of 333 at 4096: 68 us in place of 61)
   const u64 blocks = (u64)all * j_blocks * a.n_limbs * c.nrep;
   u32 tiles = 1;
-  while (tiles < 8 && blocks / (2 * tiles) >= 2048) tiles *= 2;
+  while (tiles < 8 && blocks / (2 * tiles) >= 1024) tiles *= 2;
   const dim3 grid((all + tiles - 1) / tiles * j_blocks, a.n_limbs, c.nrep), block(64 * WJ * WN);
   if constexpr (MT * WJ > 2) {  // (linear_pack_outputs)
     if (a.packed) {
@@ -424,6 +432,10 @@ void launch_linear_i8(const DevCtx& c, const LinearArgs& a, hipStream_t s) {
   if (!linear_fits(c, a)) {
     const u32 n_blocks = (c.N + 255) / 256, j_blocks = (a.n_out + kJ - 1) / kJ;
     hipLaunchKernelGGL(linear_i8_kernel, dim3(n_blocks * j_blocks * a.n_comp * a.rows, a.n_limbs, c.nrep), dim3(256), 0, s, c, a, n_blocks, j_blocks);
+  // Waves along the outputs first, then along the columns: a thread then stages one or two column blocks, and what it holds of the inputs in flight
+  // stays in registers (four blocks, <4, 1, 4> for 33 .. 64 outputs, spill: 141 -> 48 at N = 16384 237 us in place of 81; 141 -> 20 by <2, 1, 4> 80
+  // in place of 58).  Above 128 outputs three or four tiles a wave, whichever leaves fewer idle: 333 -> 300 at 2048 64 us by three, 76 by four.
+  // Two for all widths read the inputs more often (768 -> 2304: 2.0 ms), five do not fit the registers.
   } else if (a.n_out <= 32) {
     launch_mfma<1, 2, 2>(c, a, s);
   } else if (a.n_out <= 64) {
