@@ -515,7 +515,7 @@ class LargeAttn(Attn):
 
 
 @pytest.mark.parametrize("sizes,kind", [((2, 1, 1, 1, 5, 18), None), ((2, 1, 3, 4, 3, 9), None), ((2, 1, 9, 9, 10, 6), None), ((1, 1, 5, 66, 2, 5), None), ((1, 1, 6, 17, 33, 5), "top"),
-                                        ((1, 1, 1, 20, 33, 17), "top"), ((1, 1, 4, 9, 20, 4), "alternate")], ids=str)
+                                        ((1, 1, 1, 20, 33, 17), "top"), ((1, 1, 4, 9, 20, 4), "alternate"), ((2, 2, 13, 6, 9, 4), None)], ids=str)
 def test_linear_attention_in_large_launches(sizes, kind):
     """a launch that fills the card (a ring of 16384): rows, small and large sets of results, sums over many terms"""
     rt = _open.setdefault("n16384", A.AceHip(16384, 2, 60, 50, 1))
