@@ -71,6 +71,14 @@ struct Acc {
     const u64 x = v + (u64)(u32)((float)(u32)(v >> 32) * r.near_q) * r.nq;
     return x >= r.q ? x - r.q : x;
   }
+  // times f, as the start of further sums at primes of up to 60 bits: below 10q, whose part above 2^hb fits the room that the exact bound leaves.
+  // fp: companion of f; g = f w mod q with its companion gp
+  __device__ __forceinline__ Acc times(const Reduce<true>& r, u64 f, u64 fp, u64 g, u64 gp) const {
+    const u64 mid = mm - ll - hh + (ll >> r.hb);
+    const u64 v = mul_near(hh + (mid >> r.hb), g, gp, r.nq) + mul_near(((u64)((u32)mid & r.mask) << r.hb) | ((u32)ll & r.mask), f, fp, r.nq);
+    const u32 l = (u32)v & r.mask;
+    return Acc{l, l + (v >> r.hb), 0};
+  }
 };
 
 #define GLOBAL __attribute__((address_space(1)))
@@ -356,7 +364,10 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void linattn_shared_kernel
   };
 
   Acc s[MT][NT][3];
-  const u32 period = 1u << min(62 - P.nbits, 24u);
+  // Factors of rows (term 1) are applied to long sums at their end.  What is staged with a factor stays below 3q at primes of up to 56 bits: the upper
+  // halves and the middle parts have two bits more, so a quarter of the terms.
+  const bool late = a.scale != nullptr && a.t1.K >= 16 && P.nbits <= 60, lazy = P.nbits <= 56;
+  const u32 period = 1u << min(62 - P.nbits - (lazy && (a.decay || (a.scale && !late)) ? 2 : 0), 24u);
   u32 left = period;  // terms that the sums still take
   bool second = false;
 #pragma unroll
@@ -381,7 +392,7 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void linattn_shared_kernel
 #pragma unroll 1
   for (u32 part = 0; part < 2; ++part) {
     const LinattnTerm& t = part ? a.t2 : a.t1;
-    const bool causal = part && a.causal, weighted = part ? a.decay != nullptr : a.scale != nullptr;
+    const bool causal = part && a.causal, weighted = part ? a.decay != nullptr : a.scale && !late;
     const u32 K = causal ? (u32)min((int64_t)t.K, max(wg_last + 1, (int64_t)0)) : t.K;  // of the workgroup; K_own: of this wave's results
     const u32 K_own = idle ? 0 : causal ? (u32)min((int64_t)t.K, max(last + 1, (int64_t)0)) : t.K;
     if (K == 0) continue;
@@ -441,6 +452,7 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void linattn_shared_kernel
 #pragma unroll
               for (int p = 0; p < 2; ++p) {
                 v[p] = v[p] * f.x - mulhi64(v[p], f.y) * q;  // (the companion is at most one too small: below 3q)
+                if (lazy) continue;
                 v[p] = v[p] >= 2 * q ? v[p] - 2 * q : v[p];
                 v[p] = v[p] >= q ? v[p] - q : v[p];
               }
@@ -497,6 +509,22 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void linattn_shared_kernel
         }
       }
       buf ^= 1u;
+    }
+    if (part == 0 && late) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const u64 f = signed_mod(reb(c, a.scale, rep)[h * a.M + min(m0 + i, a.M - 1)], q, mh), fp = f * mh + mulhi64(f, P.prec128_lo);
+        u64 g = f * red.w - mulhi64(f, red.wp) * q;  // (below 4q)
+        g = g >= 2 * q ? g - 2 * q : g;
+        g = g >= q ? g - q : g;
+        const u64 gp = g * mh + mulhi64(g, P.prec128_lo);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int p = 0; p < 3; ++p) s[i][j][p] = s[i][j][p].times(red, f, fp, g, gp);
+      }
+      left = period;
+      second = false;
     }
   }
   u64* y = reb(c, a.out.d, rep) + h * a.out.head + limb;

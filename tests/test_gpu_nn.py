@@ -531,6 +531,19 @@ def test_linear_attention_in_large_launches(sizes, kind):
     a.free()
 
 
+@pytest.mark.parametrize("kind", [None, "top"])
+@pytest.mark.parametrize("sizes", [(1, 1, 5, 40, 17, 5), (1, 1, 2, 70, 40, 3)], ids=str)
+def test_linear_attention_long_sums_at_56_bits(sizes, kind):
+    """factors staged without their last reduction, sums that carry in between, row factors at the end of a sum or at its terms"""
+    for name, cls in (("n16384_56", LargeAttn), ("n1024_56", Attn)):
+        rt = _open.setdefault(name, A.AceHip(16384 if cls is LargeAttn else 1024, 2, 60, 56, 1))
+        a = cls(rt, 2, [0, 1], *(sizes if cls is LargeAttn else (1, 1, 2, 40, 17, 2)), kind=kind)
+        a.out()
+        a.out(causal=False)
+        a.state()
+        a.free()
+
+
 @pytest.mark.parametrize("orders", [("rhcp",) * 6, ("pcrh",) * 6, ("rhcp", "cprh", "rhcp", "hcrp", "hprc", "hrpc")], ids=str)
 @pytest.mark.parametrize("pad", [0, 1])
 def test_linear_attention_layouts(contexts, orders, pad):
