@@ -273,10 +273,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linattn_kernel(DevCtx c, Lina
 
 // The same with the operands of a workgroup's waves shared through LDS: every row of A and column of B is read by one wave, has its factor and mask
 // applied and its residues split in halves there, KS terms at a time and one stage ahead.
-// Bound by the integer instructions: 106 for a wave's term of 4 x 64 results (48 multiply-adds, 11 to add halves and read LDS, 15 staging, up to 40 of
-// carries at primes of 60 bits, the rest start and end of a sum of 32 terms), all at about four cycles.  32 x 32 causal scores of 32 features, four heads
-// of two, three limbs at N = 4096: 1.01 ms, 10^10 multiply-adds (30 % of the rate they reach alone), 1.8 GB.  One token into 32 x 32 states, four
-// heads and limbs at 8192: 1.27 ms for 5.5 GB (4.3 TB/s), bound by memory.
+// Bound by the integer instructions, at about four cycles each: 100 for a wave's term of 4 x 64 results without factors (48 multiply-adds, 10 to add halves and
+// read LDS, 14 staging, up to 36 of carries at primes of 60 bits, the rest start and end of a sum of 32 terms), 60 in place of 14 where the staged
+// residues have factors.  32 x 32 causal scores of 32 features, four heads of two, three limbs at N = 4096: 0.90 ms, 10^10 multiply-adds (38 % of the
+// rate they reach alone), 1.8 GB.  A chunk of 16 with a state of 24 x 32, two heads, three limbs at 8192: 1.01 ms, the units for them busy for 85 % of it.
+// One token into 32 x 32 states, four heads and limbs at 8192: 1.27 ms for 5.5 GB (4.3 TB/s), bound by memory.
 // Sums of int8 products on the matrix cores, as in linear.hip, cost as many instructions: tiles of 16 x 16 leave a byte 16 uses for its transposition,
 // and the reductions at the end weigh more at sums this short; that form took 1.63 ms.
 // Tiles of 2 x 2 results in 2 x 2 waves: 2 x 4 results (half the waves) 1.56 ms, 2 x 4 waves 1.52, two terms a stage 1.16.
@@ -286,7 +287,7 @@ __device__ __forceinline__ void lds_barrier() {  // LDS writes are visible, requ
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 // The tiles of a launch, row by row, without those of causal scores that no query sees (workgroups that end at once come in a pattern that leaves some
-// of the shader engines, which take workgroups in turn, without work: 32 x 32 scores 1.01 ms in place of 0.85).  Row tm of tiles has
+// of the shader engines, which take workgroups in turn, without work: 32 x 32 scores 1.01 ms in place of 0.90).  Row tm of tiles has
 // tm + lead of them, between 0 and n: rows r0 .. r0 + grow - 1 have c0, c0 + 1, ..; the rows behind all n.
 struct Tiles {
   u32 all, n, r0 = 0, c0 = 0, grow = 0;
@@ -364,9 +365,10 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void linattn_shared_kernel
   };
 
   Acc s[MT][NT][3];
-  // Factors of rows (term 1) are applied to long sums at their end.  What is staged with a factor stays below 3q at primes of up to 56 bits: the upper
-  // halves and the middle parts have two bits more, so a quarter of the terms.
-  const bool late = a.scale != nullptr && a.t1.K >= 16 && P.nbits <= 60, lazy = P.nbits <= 56;
+  // Factors of rows (term 1) are applied to long sums at their end (chunks of 16, 32 columns, two heads, three limbs at N = 8192: 8 terms 670 us, 662 staged;
+  // 12 terms 753 and 761, 48 terms 1.51 and 1.74 ms).  What is staged with a factor stays below 3q at primes of up to 56 bits: the upper halves and the
+  // middle parts have two bits more, so a quarter of the terms between carries.
+  const bool late = a.scale != nullptr && a.t1.K >= 12 && P.nbits <= 60, lazy = P.nbits <= 56;
   const u32 period = 1u << min(62 - P.nbits - (lazy && (a.decay || (a.scale && !late)) ? 2 : 0), 24u);
   u32 left = period;  // terms that the sums still take
   bool second = false;
