@@ -194,6 +194,7 @@ int acehip_rope_messages(acehip_ctx* c, double* d_cos, double* d_sin, size_t out
   if (!c) return fail(ACEHIP_EINVAL, "null context");
   if (n_axes > ROPE_AXES_MAX) return k.bad("more than eight axes");
   if (n_pairs > 65535) return k.bad("more than 65535 pairs");
+  if (n_pos >> 31) return k.bad("2^31 or more positions");
   if (n_pos == 0 || n_pairs == 0) return check_dev(c);
   if (!d_cos || !d_sin || !d_pos || !h_freq || !h_axis) return k.bad("null argument");
   for (u32 i = 0; i < n_pairs; ++i)

@@ -374,7 +374,7 @@ int acehip_linear_i8(acehip_ctx* ctx, const acehip_mat* out, const acehip_mat* i
 /* Rotary positions with several axes (time, height, width ...): pair i of features turns by pos[axis[i]][t] * freq[i] at token t.
  * acehip_rope_messages writes the messages of the tables, d_cos / d_sin[i*out_stride + t] for i < n_pairs, t < n_pos, as doubles
  * (acehip_encode[_batch] kind 1 makes plaintexts of them).  d_pos: [n_axes][pos_stride] doubles; h_freq, h_axis: HOST arrays of n_pairs,
- * axis indices below n_axes <= 8.  The angle is the rounded product of the two doubles. */
+ * axis indices below n_axes <= 8; n_pos < 2^31.  The angle is the rounded product of the two doubles. */
 int acehip_rope_messages(acehip_ctx* ctx, double* d_cos, double* d_sin, size_t out_stride, const double* d_pos, size_t pos_stride, uint32_t n_pos,
                          const double* h_freq, const uint32_t* h_axis, uint32_t n_pairs, uint32_t n_axes, acehip_stream stream);
 /* acehip_rope turns the encrypted features: of pair i < dim/2 of every head and row,

@@ -208,7 +208,7 @@ def test_rope(rt):
 
 def test_rope_messages(rt):
     for bad in (dict(axes=9), dict(axes=2), dict(axes=0), dict(cos=None), dict(sin=None), dict(pos=None), dict(freq=None), dict(axis=None), dict(os=9), dict(cos=BASE + 4),
-                dict(sin=BASE + 8), dict(pos=BASE + 16), dict(pos=BASE + FAR - 8), dict(pairs=65536), dict(os=1 << 61)):
+                dict(sin=BASE + 8), dict(pos=BASE + 16), dict(pos=BASE + FAR - 8), dict(pairs=65536), dict(os=1 << 61), dict(n=1 << 31, os=1 << 31, cos=1 << 50, sin=1 << 51, pos=1 << 52)):
         assert changed(Messages, **bad).call(rt) == EINVAL, bad
     for good in (dict(n=0), dict(pairs=0), dict(ps=0), dict(pairs=1, os=0)):
         assert changed(Messages, **good).call(rt) == ENODEV, (good, rt.err())
