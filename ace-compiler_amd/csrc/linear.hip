@@ -110,9 +110,10 @@ __device__ __forceinline__ void linear_tiles(const DevCtx& c, const LinearArgs& 
   // addresses: a uniform 64-bit base that moves with the step plus 32-bit offsets of the lanes that stay (linear_fits)
   const u64 xs = a.in.col;
   const u32 k4 = (t >> 4) & 15u, u0 = t >> 8;  // this thread stages inputs 4 k4 .. 4 k4 + 3 of a step in column blocks u0, u0 + WN / G ..
+  const u32 k_wave = 16 * (wave & 3u);         // the first of its wave's 16 inputs: the base is the wave's
   u32 x_at[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x_at[i] = 8 * ((4 * k4 + i) * (u32)xs + u0 * 16 + (t & 15u));
+  for (int i = 0; i < 4; ++i) x_at[i] = 8 * ((4 * (lane >> 4) + i) * (u32)xs + u0 * 16 + (t & 15u));
   const GLOBAL char* w = (const GLOBAL char*)global(uniform(PACKED ? (const int8_t*)a.packed : reb(c, a.w, rep) + (u64)j0 * a.ld_w));
   u32 w_at[MT];  // of the lane's row; packed: of the fragments' tile, in steps
 #pragma unroll
@@ -127,12 +128,13 @@ __device__ __forceinline__ void linear_tiles(const DevCtx& c, const LinearArgs& 
   // behind the last tile nothing is read.  No branch (the steps are one block of code): x_next is made ready once a tile.
   u32 x_tile = 0, x_step = 0, any_row;
   u64 any_off;
-  int x_rest = (int)a.n_in;
-  const int limb64 = (int)xs * 512;  // bytes of a whole step
-  const u64* x = block(0, a.in, x_base, any_row, any_off);
-  const u64* x_next = block(1, a.in, x_base, any_row, any_off);
+  const int x_all = (int)a.n_in - (int)k_wave;
+  int x_rest = x_all;
+  const int limb16 = (int)xs * 128;
+  const u64* x = block(0, a.in, x_base, any_row, any_off) + k_wave * xs;
+  const u64* x_next = block(1, a.in, x_base, any_row, any_off) + k_wave * xs;
   auto load_x = [&](Raw& r) {
-    const int bytes = x_rest >= 64 ? limb64 : x_rest > 0 ? x_rest * (int)xs * 8 : 0;
+    const int bytes = x_rest >= 16 ? limb16 : x_rest > 0 ? x_rest * (int)xs * 8 : 0;
     const auto d = __builtin_amdgcn_make_buffer_rsrc((void*)x, 0, bytes, 0x00027000);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -141,7 +143,7 @@ __device__ __forceinline__ void linear_tiles(const DevCtx& c, const LinearArgs& 
     const bool wrap = x_step == (last | 1u);
     x_step = wrap ? 0 : x_step + 1;
     x_tile += wrap;
-    x_rest = wrap ? (x_tile < cols.n ? (int)a.n_in : 0) : x_rest - 64;
+    x_rest = wrap ? (x_tile < cols.n ? x_all : 0) : x_rest - 64;
     x = wrap ? x_next : x + 64 * xs;
   };
   auto stage = [&](const Raw& r, v4i_t* buf) {
@@ -231,7 +233,7 @@ __device__ __forceinline__ void linear_tiles(const DevCtx& c, const LinearArgs& 
   u64 off, tok = 0;
   GLOBAL char* y;
   auto begin = [&] {
-    x_next = block(x_tile + 1, a.in, x_base, any_row, any_off);
+    x_next = block(x_tile + 1, a.in, x_base, any_row, any_off) + k_wave * xs;
     y = (GLOBAL char*)global(block(tile, a.out, y_base, row, off) + (u64)(j0 + wj * MT * 16) * a.out.col);
     y = (GLOBAL char*)uniform((char*)y);
     if (a.tok) tok = global(uniform(reb(c, a.tok, rep) + row * a.tok_stride + off))[n];
@@ -347,7 +349,7 @@ __global__ __launch_bounds__(64 * WJ * WN, 2) void linear_i8_mfma_kernel(DevCtx 
   else                linear_tiles<8, MT, WJ, WN, PACKED>(c, a, frag, factor, P, rep, pos, cols, j0);
 }
 
-// What the matrix-core form does not take (linear_fits: rings below 64, primes below 2^40, inputs that share words or lie over 32 MiB apart): one
+// What the matrix-core form does not take (linear_fits: rings below 64, primes below 2^40, inputs that share words or lie 128 MiB apart): one
 // coefficient per lane, kJ outputs, residues split at 31 bits, so that each half times a weight is one multiply-add into a signed 64-bit sum (|sum| <= 2^31 * 2^7 * 2^16 inputs).
 constexpr u32 kJ = 8;
 __global__ __launch_bounds__(256) void linear_i8_kernel(DevCtx c, LinearArgs a, u32 n_blocks, u32 j_blocks) {
@@ -391,7 +393,7 @@ __global__ __launch_bounds__(256) void linear_i8_kernel(DevCtx c, LinearArgs a, 
 // the matrix-core form: rings and primes that it takes, inputs that lie apart (a descriptor that ends behind the last one reads zeros for those past
 // it), lane offsets below 2^32, and an array of weights that holds a fragment of 16 bytes
 static bool linear_fits(const DevCtx& c, const LinearArgs& a) {
-  return c.N >= 64 && a.wide_primes && a.in.col >= c.N && a.in.col <= (1u << 22) && a.out.col <= (1u << 23) && a.ld_w <= (1u << 24) && a.n_in != 0 &&
+  return c.N >= 64 && a.wide_primes && a.in.col >= c.N && a.in.col < (1u << 24) && a.out.col < (1u << 25) && a.ld_w <= (1u << 24) && a.n_in != 0 &&
          (u64)(a.n_out - 1) * a.ld_w + a.n_in >= 16;
 }
 

@@ -225,6 +225,12 @@ def test_linear_many_column_blocks(contexts, n_in, n_out, rows, n_comp):
         d.free()
 
 
+@pytest.mark.parametrize("apart", [(1 << 22) + 64, (1 << 24) - 192 - 64, 1 << 24])
+def test_linear_far_inputs(contexts, apart):
+    """ciphertexts 32 and 128 MiB apart"""
+    linear_case(contexts("n64"), 3, [0, 1, 2], 1, 3, 2, 1, True, pad=apart)
+
+
 @pytest.mark.parametrize("same", ["row", "col", "comp", "all"])
 @pytest.mark.parametrize("n_in,n_out", [(5, 3), (70, 40)])
 def test_linear_shared_inputs(contexts, same, n_in, n_out):
