@@ -91,8 +91,8 @@ __device__ __forceinline__ const GLOBAL char* uniform(const u64* p) {
 // A wave: 64 coefficients, MT x NT results (3 sums of 3 words each); a workgroup: WM x WN such tiles of the same coefficients, whose operands
 // meet in the CU's L1.  Per term of the sums a lane reads 2 (MT + NT) residues and makes 12 MT NT multiply-adds.
 // WIDE: primes above 2^32 (the reduction's quotient from three partial products).
-// In use for one row of results, where nothing but the row is read twice: bound by memory (32 x 32 states read by one token, two heads and limbs at N = 1024,
-// 10 us from the caches; 48 x 48, four heads, three limbs at 8192: 3.8 GB in 0.72 ms, 5.3 TB/s), and for the chains and rings that the form below does not take.
+// In use for one row of results, where nothing but the row is read twice: bound by memory (48 x 48 states read by one token, four heads, three limbs at
+// N = 8192: 3.8 GB in 0.72 ms, 5.3 TB/s); and for the chains and rings that the form below does not take.
 template <int MT, int NT, int WM, int WN, bool WIDE>
 __global__ __launch_bounds__(64 * WM * WN, 2) void linattn_kernel(DevCtx c, LinattnArgs a, u32 n_blocks, u32 m_tiles, u32 n_tiles) {
   constexpr u32 KC = 64;  // terms whose factors are prepared at a time

@@ -16,7 +16,7 @@ namespace acehip {
 // as the B fragments of v_mfma_i32_16x16x64_i8 (1 KiB each, read without bank conflicts); the weights are the A fragments, packed by a kernel of
 // their own (or, up to 32 outputs, as their rows lie in memory).  Residues are requested three steps ahead and staged one ahead, weights one.
 // Bound: up to 128 outputs by memory (800 -> 32, N = 16384, two rows, three limbs: 0.28 ms, 4.7 TB/s; 333 -> 77, N = 4096, three rows: 59 us, 4.1 TB/s);
-// above by the matrix cores and the power that they draw (768 -> 2304 at N = 16384: 1.64 ms, 2.78 * 10^15 int8 operations, 1.70 POP/s; the product
+// above by the matrix cores and the power that they draw (768 -> 2304 at N = 16384: 1.66 ms, 2.78 * 10^15 int8 operations, 1.67 POP/s; the product
 // with its LDS reads and stores alone takes 0.92 ms, staging 0.15, the loads 0.4 and the reduction 0.2: the parts add up since the clock falls to
 // 1.96 GHz; a library's int8 product of 8192^3 reaches 2.08 POP/s on this card).
 // ------------------------------------------------------------------------------------------------
@@ -350,7 +350,8 @@ __global__ __launch_bounds__(64 * WJ * WN, 2) void linear_i8_mfma_kernel(DevCtx 
 }
 
 // What the matrix-core form does not take (linear_fits: rings below 64, primes below 2^40, inputs that share words or lie 128 MiB apart): one
-// coefficient per lane, kJ outputs, residues split at 31 bits, so that each half times a weight is one multiply-add into a signed 64-bit sum (|sum| <= 2^31 * 2^7 * 2^16 inputs).
+// coefficient per lane, kJ outputs, residues split at 31 bits, so that each half times a weight is one multiply-add into a signed 64-bit sum
+// (|sum| <= 2^31 * 2^7 * 2^16 inputs).
 constexpr u32 kJ = 8;
 __global__ __launch_bounds__(256) void linear_i8_kernel(DevCtx c, LinearArgs a, u32 n_blocks, u32 j_blocks) {
   u32 b = blockIdx.x;
