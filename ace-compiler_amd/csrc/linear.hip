@@ -59,20 +59,14 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const int8_t* w, u64 l
   const u32 f = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63u;
   if (f >= n_frags) return;
   const u32 j = (f / steps) * 16 + (lane & 15u), k = (f % steps) * 64 + 16 * (lane >> 4);
-  v4i_t v{0, 0, 0, 0};
+  // 16 bytes from the array, the last ones of it at most (linear_fits: it has 16), moved to their place; those past the row are cleared
+  unsigned __int128 v = 0;
   if (j < n_out && k < n_in) {
-    const GLOBAL int8_t* p = global(w) + j * ld_w + k;
-    if (k + 16 <= n_in) {
-      v = *(const GLOBAL v4i_any_t*)p;
-    } else {
-#pragma unroll
-      for (int d = 0; d < 4; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (k + 4 * d + i < n_in) v[d] |= (int)((u32)(uint8_t)p[4 * d + i] << (8 * i));
-    }
+    const u64 at = j * ld_w + k, last = (n_out - 1) * ld_w + n_in - 16, from = min(at, last);
+    v = __builtin_bit_cast(unsigned __int128, (v4i_t) * (const GLOBAL v4i_any_t*)(global(w) + from)) >> (8 * (u32)(at - from));
+    if (n_in - k < 16) v &= ((unsigned __int128)1 << (8 * (n_in - k))) - 1;
   }
-  out[(u64)f * 64 + lane] = v;
+  out[(u64)f * 64 + lane] = __builtin_bit_cast(v4i_t, v);
 }
 
 // a * w mod q up to multiples of q for a < 2^63, with nq = -q and a companion wp of w that is at most two units of 2^-64 too small: below 4q
