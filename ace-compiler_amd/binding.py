@@ -2,6 +2,7 @@
 HIP library; if the library is missing or there is no GPU the calls raise (no CPU fallback)."""
 import ctypes as C
 import os
+import struct
 
 import numpy as np
 
@@ -419,7 +420,7 @@ class AceHip:
         n = len(freq)
         if len(axis) != n:
             raise ValueError("as many axes as frequencies are needed")
-        self.check(self.lib.acehip_rope_messages(self.h, d_cos, d_sin, out_stride, d_pos, pos_stride, n_pos, (C.c_double * n)(*freq), (_u32 * n)(*axis), n,
+        self.check(self.lib.acehip_rope_messages(self.h, d_cos, d_sin, out_stride, d_pos, pos_stride, n_pos, struct.pack("%dd" % n, *freq), struct.pack("%dI" % n, *axis), n,
                                                  n_axes, stream))
 
     def rope(self, out, x, d_cos, d_sin, pair_stride, row_stride, n_heads, rows, dim, n_comp, level, pos0=0, n_limbs=None, interleaved=False, stream=None):

@@ -3,21 +3,28 @@
 
 namespace acehip {
 
-// The angle is one rounded product of doubles; cos and sin of that double (positions far out lose nothing more).  Bound by its stores and its launch:
-// 16384 positions of 64 pairs, 34 MB, in 8.5 us (4.0 TB/s).
+// The angle is one rounded product of doubles; cos and sin of that double (positions far out lose nothing more).  Two positions a lane, whose
+// latencies overlap.  Bound by its stores and its launch: 32768 positions of 64 pairs, 34 MB, in 7.6 us (4.5 TB/s); replayed in a graph 9.7 us, 10.4 with
+// one position a lane, 8.3 without the functions.
 __global__ __launch_bounds__(256) void rope_messages_kernel(double* cos_out, double* sin_out, u64 out_stride, const double* pos, u64 pos_stride, u32 n_pos,
                                                             RopeAngles a) {
-  const u32 t = blockIdx.x * 256 + threadIdx.x, i = blockIdx.y;
-  if (t >= n_pos) return;
-  double s, c;
-  sincos(pos[a.axis[i] * pos_stride + t] * a.freq[i], &s, &c);
-  cos_out[i * out_stride + t] = c;
-  sin_out[i * out_stride + t] = s;
+  const u32 i = blockIdx.y, t0 = blockIdx.x * 512 + threadIdx.x;
+  const double* p = pos + a.axis[i] * pos_stride;
+  double s[2], c[2];
+#pragma unroll
+  for (u32 u = 0; u < 2; ++u) sincos(p[min(t0 + 256 * u, n_pos - 1)] * a.freq[i], &s[u], &c[u]);
+#pragma unroll
+  for (u32 u = 0; u < 2; ++u) {
+    const u32 t = t0 + 256 * u;
+    if (t >= n_pos) return;
+    cos_out[i * out_stride + t] = c[u];
+    sin_out[i * out_stride + t] = s[u];
+  }
 }
 
 void launch_rope_messages(double* cos_out, double* sin_out, u64 out_stride, const double* pos, u64 pos_stride, u32 n_pos, const RopeAngles& a, u32 n_pairs,
                           hipStream_t s) {
-  hipLaunchKernelGGL(rope_messages_kernel, dim3((n_pos + 255) / 256, n_pairs), dim3(256), 0, s, cos_out, sin_out, out_stride, pos, pos_stride, n_pos, a);
+  hipLaunchKernelGGL(rope_messages_kernel, dim3((n_pos + 511) / 512, n_pairs), dim3(256), 0, s, cos_out, sin_out, out_stride, pos, pos_stride, n_pos, a);
 }
 
 // A lane: one coefficient of a pair, whose table it reads once for up to `per` polynomials (heads and components); `parts` workgroups share a
