@@ -88,119 +88,107 @@ __device__ __forceinline__ const GLOBAL char* uniform(const u64* p) {
   return (const GLOBAL char*)(((u64)(u32)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) | (u32)__builtin_amdgcn_readfirstlane((int)v));
 }
 
-// A wave: 64 coefficients, MT x NT results (3 sums of 3 words each); a workgroup: WM x WN such tiles of the same coefficients, whose operands
-// meet in the CU's L1.  Per term of the sums a lane reads 2 (MT + NT) residues and makes 12 MT NT multiply-adds.
+// One row of results.  A wave: 64 coefficients, NT results (3 sums of 3 words each) over every KW-th term; a workgroup: WN waves along the columns, KW along
+// the terms, whose sums are joined through LDS.  Per term of the sums a lane reads 2 (1 + NT) residues and makes 12 NT multiply-adds.
 // WIDE: primes above 2^32 (the reduction's quotient from three partial products).
 // In use for one row of results, where nothing but the row is read twice: bound by memory (48 x 48 states read by one token, four heads, three limbs at
-// N = 8192: 3.8 GB in 0.72 ms, 5.3 TB/s); and for the chains and rings that the form below does not take.
-template <int MT, int NT, int WM, int WN, bool WIDE>
-__global__ __launch_bounds__(64 * WM * WN, 2) void linattn_kernel(DevCtx c, LinattnArgs a, u32 n_blocks, u32 m_tiles, u32 n_tiles) {
+// N = 8192: 3.8 GB in 0.72 ms, 5.3 TB/s); for launches that leave the card empty; and for the chains and rings that the form below does not take.
+template <int NT, int WN, int KW, bool WIDE>
+__global__ __launch_bounds__(64 * WN * KW, 2) void linattn_kernel(DevCtx c, LinattnArgs a, u32 n_blocks, u32 n_tiles) {
   constexpr u32 KC = 64;  // terms whose factors are prepared at a time
-  __shared__ ulong2 factor[KC + MT * WM];
+  static_assert(KC % KW == 0 && (KW == 1 || WN == 1), "a wave keeps its place among the terms, a workgroup of several ends as one");
+  __shared__ ulong2 factor[KC];
+  __shared__ u64 joined[KW == 1 ? 1 : KW - 1][NT * 9][64];
   u32 b = blockIdx.x;
   // tiles of the same coefficients follow each other on one XCD (ids congruent mod 8): its L2 keeps their operands
-  const u32 groups = gridDim.x / (m_tiles * n_tiles);
+  const u32 tiles = a.M * n_tiles, groups = gridDim.x / tiles;
   u32 g, t;
   if ((groups & 7u) == 0) {
     const u32 x = b >> 3;
-    t = x % (m_tiles * n_tiles);
-    g = (x / (m_tiles * n_tiles)) * 8 + (b & 7u);
+    t = x % tiles;
+    g = (x / tiles) * 8 + (b & 7u);
   } else {
-    t = b % (m_tiles * n_tiles);
-    g = b / (m_tiles * n_tiles);
+    t = b % tiles;
+    g = b / tiles;
   }
   t = __builtin_amdgcn_readfirstlane(t);
   g = __builtin_amdgcn_readfirstlane(g);
   const u32 nb = g & (n_blocks - 1), h = g >> __builtin_ctz(n_blocks), rep = c.rep0 + blockIdx.z;
-  const u32 lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const u32 wg_m = (t / n_tiles) * (MT * WM), m0 = wg_m + (wave / WN) * MT, j0 = ((t % n_tiles) * WN + wave % WN) * NT;
+  const u32 lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = wave / WN;
+  const u32 row = t / n_tiles, j0 = ((t % n_tiles) * WN + wave % WN) * NT;
   const u32 pos = a.pos0 + blockIdx.y, gi = limb_prime(pos, a.level, c.L);
   if (!owns(c, gi)) return;
-  const int64_t off = a.off;
-  // last column / key that the rows of the workgroup and of this wave see (rows past M: the last one's)
-  const int64_t wg_last = (int64_t)min(wg_m + MT * WM, a.M) - 1 + off, last = (int64_t)min(m0 + MT, a.M) - 1 + off;
-  if (a.skip_above && (int64_t)j0 > last) return;  // (scores: no factors, so no barrier to meet)
+  const int64_t last = (int64_t)row + a.off;  // column / key that the row sees
+  if (a.skip_above && (int64_t)j0 > last) return;  // (scores: no factors, so no barrier to meet before the joint one)
   const DevPrime P = c.primes[gi];
   const Reduce<WIDE> red(P);
   const u64 q = P.q, mh = P.prec128_hi;
   const u32 hb = red.hb;
   const u32 n = nb * 64 + lane, at = 8 * min(n, c.N - 1);  // (rings below 64: the lanes behind the ring repeat its last coefficient and store nothing)
   const u64 limb = (u64)pos * c.N;
-  u32 row[MT], col[NT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) row[i] = min(m0 + i, a.M - 1);
+  u32 col[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) col[i] = min(j0 + i, a.Nn - 1);
   auto read = [&](const u64* p) { return *(const GLOBAL u64*)(uniform(p) + at); };
 
-  Acc s[MT][NT][3];
+  Acc s[NT][3];
   const u32 period = 1u << min(62 - P.nbits, 24u);
   u32 left = period;  // terms that the sums still take
   bool second = false;
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
+  for (int j = 0; j < NT; ++j)
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int p = 0; p < 3; ++p) s[i][j][p] = Acc{0, 0, 0};
-  if (a.base.d) {  // one term: keep * base
+    for (int p = 0; p < 3; ++p) s[j][p] = Acc{0, 0, 0};
+  if (a.base.d && wk == 0) {  // one term: keep * base
     const u64* S = reb(c, a.base.d, rep) + h * a.base.head + limb;
     const Half f = halves(a.keep ? signed_mod(reb(c, a.keep, rep)[h], q, mh) : 1, hb);
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int p = 0; p < 2; ++p) s[i][j][p].mac(halves(read(S + row[i] * a.base.row + col[j] * a.base.col + p * a.base.comp), hb), f);
+      for (int p = 0; p < 2; ++p) s[j][p].mac(halves(read(S + row * a.base.row + col[j] * a.base.col + p * a.base.comp), hb), f);
     --left;
   }
   struct Raw {
-    u64 a[MT][2], b[NT][2];
+    u64 a[2], b[NT][2];
   };
 #pragma unroll 1
   for (u32 part = 0; part < 2; ++part) {
     const LinattnTerm& t = part ? a.t2 : a.t1;
-    const bool causal = part && a.causal, weighted = part ? a.decay != nullptr : a.scale != nullptr;
-    // a causal sum ends with the last key that a row of the wave (of the workgroup: the factors) sees
-    const u32 K = causal ? (u32)min((int64_t)t.K, max(last + 1, (int64_t)0)) : t.K, K_wg = causal ? (u32)min((int64_t)t.K, max(wg_last + 1, (int64_t)0)) : t.K;
-    if (K_wg == 0) continue;
-    const u64* A = reb(c, t.a.d, rep) + (t.a_group == 1 ? h : h / t.a_group) * t.a.head + limb;
-    const u64* B = reb(c, t.b.d, rep) + (t.b_group == 1 ? h : h / t.b_group) * t.b.head + limb;
-    const u64 a_col = t.a.col, b_row = t.b.row;
-    const u64 *pa[MT][2], *pb[NT][2];  // where the next term's residues lie
+    const bool weighted = part ? a.decay != nullptr : a.scale != nullptr;
+    const u32 K = part && a.causal ? (u32)min((int64_t)t.K, max(last + 1, (int64_t)0)) : t.K;  // a causal sum ends with the last key that the row sees
+    if (K == 0) continue;
+    const u32 k_first = min(wk, K - 1);
+    const u64* A = reb(c, t.a.d, rep) + (t.a_group == 1 ? h : h / t.a_group) * t.a.head + limb + row * t.a.row + k_first * t.a.col;
+    const u64* B = reb(c, t.b.d, rep) + (t.b_group == 1 ? h : h / t.b_group) * t.b.head + limb + k_first * t.b.row;
+    const u64 a_next = KW * t.a.col, b_next = KW * t.b.row;
+    const u64 *pa[2], *pb[NT][2];  // where the wave's next term's residues lie
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int p = 0; p < 2; ++p) pa[i][p] = A + row[i] * t.a.row + p * t.a.comp;
+    for (int p = 0; p < 2; ++p) pa[p] = A + p * t.a.comp;
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int p = 0; p < 2; ++p) pb[i][p] = B + col[i] * t.b.col + p * t.b.comp;
     auto load = [&](Raw& r, bool more) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          r.a[i][p] = read(pa[i][p]);
-          pa[i][p] += more ? a_col : 0;
-        }
+      for (int p = 0; p < 2; ++p) {
+        r.a[p] = read(pa[p]);
+        pa[p] += more ? a_next : 0;
+      }
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
           r.b[i][p] = read(pb[i][p]);
-          pb[i][p] += more ? b_row : 0;
+          pb[i][p] += more ? b_next : 0;
         }
     };
     Raw next;
-    load(next, K > 1);
-    for (u32 k0 = 0; k0 < K_wg; k0 += KC) {
-      if (weighted) {
-        // factors of the terms from k0 on: term 1's by row; term 2's by term, or by distance (entry e: the distance that row wg_m meets at term
-        // k0 + KC - 1, and so on upwards)
+    load(next, wk + KW < K);
+    for (u32 k0 = 0; k0 < K; k0 += KC) {
+      if (weighted) {  // factors of the terms from k0 on: term 1's of the row, term 2's by term or by distance
         __syncthreads();
-        for (u32 e = threadIdx.x; e < KC + MT * WM; e += 64 * WM * WN) {
-          const int64_t d = part == 0 ? (int64_t)min(wg_m + e, a.M - 1) : a.decay_by_k ? (int64_t)t.K - 1 - k0 - e : (int64_t)wg_m + off - (k0 + KC - 1) + e;
+        for (u32 e = threadIdx.x; e < KC; e += 64 * WN * KW) {
+          const int64_t d = part == 0 ? (int64_t)row : a.decay_by_k ? (int64_t)t.K - 1 - k0 - e : last - k0 - e;
           const bool there = d >= 0 && d < (int64_t)(part ? t.K : a.M);
           const u64 f = there ? signed_mod(part ? reb(c, a.decay, rep)[h * a.decay_ld + d] : reb(c, a.scale, rep)[h * a.M + d], q, mh) : 0;
           factor[e] = ulong2{f, f * mh + mulhi64(f, P.prec128_lo)};
@@ -209,66 +197,74 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linattn_kernel(DevCtx c, Lina
       }
       const u32 k1 = min(k0 + KC, K);
 #pragma unroll 1
-      for (u32 k = k0; k < k1; ++k) {
+      for (u32 k = k0 + wk; k < k1; k += KW) {
         Raw r = next;
-        load(next, k + 2 < K);
+        load(next, k + 2 * KW < K);
         if (left == 0) {
 #pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              s[i][j][1].carry(red);
-              if (second) s[i][j][0].carry(red), s[i][j][2].carry(red);
-            }
+          for (int j = 0; j < NT; ++j) {
+            s[j][1].carry(red);
+            if (second) s[j][0].carry(red), s[j][2].carry(red);
+          }
           second = !second;
           left = period;
         }
         --left;
         if (weighted) {
+          const ulong2 f = factor[k - k0];
 #pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            const ulong2 f = factor[part == 0 ? row[i] - wg_m : a.decay_by_k ? k - k0 : KC - 1 - (k - k0) + (row[i] - wg_m)];
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
-              u64 v = r.a[i][p] * f.x - mulhi64(r.a[i][p], f.y) * q;  // (the companion is at most one too small: below 3q)
-              v = v >= 2 * q ? v - 2 * q : v;
-              r.a[i][p] = v >= q ? v - q : v;
-            }
+          for (int p = 0; p < 2; ++p) {
+            u64 v = r.a[p] * f.x - mulhi64(r.a[p], f.y) * q;  // (the companion is at most one too small: below 3q)
+            v = v >= 2 * q ? v - 2 * q : v;
+            r.a[p] = v >= q ? v - q : v;
           }
         }
-        if (causal && !weighted) {  // (weighted: a factor of zero)
+        const Half h0 = halves(r.a[0], hb), h1 = halves(r.a[1], hb);
 #pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int p = 0; p < 2; ++p) r.a[i][p] = (int64_t)k <= (int64_t)row[i] + off ? r.a[i][p] : 0;
-        }
-        Half bh[NT][2];
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-          for (int p = 0; p < 2; ++p) bh[i][p] = halves(r.b[i][p], hb);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          const Half h0 = halves(r.a[i][0], hb), h1 = halves(r.a[i][1], hb);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            s[i][j][0].mac(h0, bh[j][0]);
-            s[i][j][1].mac(h0, bh[j][1]);
-            s[i][j][1].mac(h1, bh[j][0]);
-            s[i][j][2].mac(h1, bh[j][1]);
-          }
+        for (int j = 0; j < NT; ++j) {
+          const Half b0 = halves(r.b[j][0], hb), b1 = halves(r.b[j][1], hb);
+          s[j][0].mac(h0, b0);
+          s[j][1].mac(h0, b1);
+          s[j][1].mac(h1, b0);
+          s[j][2].mac(h1, b1);
         }
       }
     }
   }
-  u64* y = reb(c, a.out.d, rep) + h * a.out.head + limb;
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
+  if (KW > 1) {  // joint sums: below 3q from each wave after a carry, so three fit at primes of up to 2^64 / 9
 #pragma unroll
     for (int j = 0; j < NT; ++j)
-      if (m0 + i < a.M && j0 + j < a.Nn && n < c.N && (!a.skip_above || (int64_t)(j0 + j) <= (int64_t)(m0 + i) + off))
 #pragma unroll
-        for (int p = 0; p < 3; ++p) *(GLOBAL u64*)((GLOBAL char*)uniform(y + row[i] * a.out.row + col[j] * a.out.col + p * a.out.comp) + at) = s[i][j][p].value(red);
+      for (int p = 0; p < 3; ++p) {
+        s[j][p].carry(red);
+        if (wk > 0) {
+          u64(*to)[64] = &joined[wk - 1][9 * j + 3 * p];
+          to[0][lane] = s[j][p].ll;
+          to[1][lane] = s[j][p].mm;
+          to[2][lane] = s[j][p].hh;
+        }
+      }
+    __syncthreads();
+    if (wk > 0) return;
+#pragma unroll
+    for (int w = 0; w < KW - 1; ++w)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+          const u64(*from)[64] = &joined[w][9 * j + 3 * p];
+          if (w % 2 == 0 && w) s[j][p].carry(red);
+          s[j][p].ll += from[0][lane];
+          s[j][p].mm += from[1][lane];
+          s[j][p].hh += from[2][lane];
+        }
+  }
+  u64* y = reb(c, a.out.d, rep) + h * a.out.head + limb;
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+    if (j0 + j < a.Nn && n < c.N && (!a.skip_above || (int64_t)(j0 + j) <= last))
+#pragma unroll
+      for (int p = 0; p < 3; ++p) *(GLOBAL u64*)((GLOBAL char*)uniform(y + row * a.out.row + col[j] * a.out.col + p * a.out.comp) + at) = s[j][p].value(red);
 }
 
 // The same with the operands of a workgroup's waves shared through LDS: every row of A and column of B is read by one wave, has its factor and mask
@@ -540,11 +536,10 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void linattn_shared_kernel
           *(GLOBAL u64*)((GLOBAL char*)uniform(y + (m0 + i) * a.out.row + (j0 + j) * a.out.col + p * a.out.comp) + at) = s[i][j][p].value(red);
 }
 
-template <int MT, int NT, int WM, int WN, bool WIDE>
-static void launch_tiles(const DevCtx& c, const LinattnArgs& a, hipStream_t s) {
-  const u32 n_blocks = (c.N + 63) / 64, m_tiles = (a.M + MT * WM - 1) / (MT * WM), n_tiles = (a.Nn + NT * WN - 1) / (NT * WN);
-  hipLaunchKernelGGL((linattn_kernel<MT, NT, WM, WN, WIDE>), dim3(n_blocks * m_tiles * n_tiles * a.n_heads, a.n_limbs, c.nrep), dim3(64 * WM * WN), 0, s, c, a,
-                     n_blocks, m_tiles, n_tiles);
+template <int NT, int WN, int KW, bool WIDE>
+static void launch_rows(const DevCtx& c, const LinattnArgs& a, hipStream_t s) {
+  const u32 n_blocks = (c.N + 63) / 64, n_tiles = (a.Nn + NT * WN - 1) / (NT * WN);
+  hipLaunchKernelGGL((linattn_kernel<NT, WN, KW, WIDE>), dim3(n_blocks * a.M * n_tiles * a.n_heads, a.n_limbs, c.nrep), dim3(64 * WN * KW), 0, s, c, a, n_blocks, n_tiles);
 }
 
 template <int MT, int NT, int WM, int WN, int KS, int MIN_WAVES>
@@ -556,18 +551,22 @@ static void launch_shared(const DevCtx& c, const LinattnArgs& a, hipStream_t s) 
                      n_blocks, tiles);
 }
 
+// Where a workgroup for each result leaves every workgroup a place (eight on each of 256 CUs), the sums are cut over its waves: 4 x 4 scores of 64 features
+// at N = 1024 8.3 us, 21 by the next form; a 64 x 64 state read by one token 15 and 25; with more of them it loses (16 x 16 states, 16 tokens: 24 us, 20).
+// Launches that leave half the places of the larger form empty take one result a wave and two terms a stage (9 x 9 scores of 51 features at 2048: 25 us, 38
+// by 2 x 2; from 512 workgroups on it loses: 8 x 8 scores of 24 features at 4096: 27 us, 24).
 // One row: its operands are read once whatever the form, and waiting for each other costs (48 x 48 state at N = 8192: 0.72 ms, 0.86 shared).  Two rows or
-// more share (2 x 40 x 4 scores at 8192: 53 us, 91 by linattn_kernel's tiles of 4 x 8; 64 x 2 state of four tokens 0.55 ms, 1.09).  Launches that leave
-// half the places for workgroups empty take one result a wave and two terms a stage (9 x 9 scores of 51 features at 2048: 25 us, 38 by 2 x 2; a 32 x 32
-// state read by one token at 1024, two heads and limbs, 18.5 us, 22.6 by rows; from 512 workgroups on it loses: 8 x 8 scores of 24 features at 4096: 27 us, 24).
+// more share (2 x 40 x 4 scores at 8192: 53 us, 91 unshared by tiles of 4 x 8; 64 x 2 state of four tokens 0.55 ms, 1.09).
 void launch_linattn(const DevCtx& c, const LinattnArgs& a, hipStream_t s) {
   const bool row = a.M == 1;
-  const u32 m = row ? 1 : 4, n = row ? 16 : 4;  // results of a workgroup below
-  const u64 groups = (u64)((c.N + 63) / 64) * ((a.M + m - 1) / m) * ((a.Nn + n - 1) / n) * a.n_heads * a.n_limbs * c.nrep;
-  if (!a.wide_primes)                 launch_tiles<1, 1, 1, 1, false>(c, a, s);
-  else if (c.N >= 64 && groups < 512) launch_shared<1, 1, 2, 2, 2, 4>(c, a, s);
-  else if (c.N >= 64 && !row)         launch_shared<2, 2, 2, 2, 1, 4>(c, a, s);
-  else                                launch_tiles<1, 4, 1, 4, true>(c, a, s);
+  const u64 blocks = (u64)((c.N + 63) / 64) * a.n_heads * a.n_limbs * c.nrep;
+  const u32 m = row ? 1 : 4, n = row ? 16 : 4;  // results of a workgroup of the larger forms
+  const u64 groups = blocks * ((a.M + m - 1) / m) * ((a.Nn + n - 1) / n);
+  if (!a.wide_primes)                                                         launch_rows<1, 1, 1, false>(c, a, s);
+  else if (blocks * a.M * a.Nn <= 2048 && (u64)a.t1.K + a.t2.K >= 16)         launch_rows<1, 1, 4, true>(c, a, s);
+  else if (c.N >= 64 && groups < 512)                                         launch_shared<1, 1, 2, 2, 2, 4>(c, a, s);
+  else if (c.N >= 64 && !row)                                                 launch_shared<2, 2, 2, 2, 1, 4>(c, a, s);
+  else                                                                        launch_rows<4, 4, 1, true>(c, a, s);
 }
 
 }  // namespace acehip

@@ -517,7 +517,15 @@ class LargeAttn(Attn):
 
     def __init__(self, *args, **kw):
         super().__init__(*args, **kw)
-        self.n = len(Sampled.AT)
+        self.n = len(self.Block.AT)
+
+
+class Sampled1024(Sampled):
+    AT = np.array([0, 1, 63, 64, 500, 1023])
+
+
+class MiddleAttn(LargeAttn):
+    Block = Sampled1024
 
 
 @pytest.mark.parametrize("sizes,kind", [((2, 1, 1, 1, 5, 18), None), ((2, 1, 3, 4, 3, 9), None), ((2, 1, 9, 9, 10, 6), None), ((1, 1, 5, 66, 2, 5), None), ((1, 1, 6, 17, 33, 5), "top"),
@@ -533,6 +541,24 @@ def test_linear_attention_in_large_launches(sizes, kind):
     a.out(state=False, factor=False)
     a.state()
     a.state(factor=False)
+    a.state(in_place=True)
+    a.free()
+
+
+@pytest.mark.parametrize("name,args", [("n1024_60", (1024, 2, 60, 59, 1)), ("n1024_56", (1024, 2, 60, 56, 1)), ("n1024", SETS["n1024"])])
+@pytest.mark.parametrize("sizes,kind", [((1, 1, 9, 9, 20, 10), None), ((2, 1, 7, 10, 13, 11), "top"), ((3, 1, 1, 70, 66, 15), None), ((1, 1, 2, 33, 40, 3), "top"), ((2, 1, 1, 1, 17, 31), None)],
+                         ids=str)
+def test_linear_attention_in_middle_launches(name, args, sizes, kind):
+    """launches that do not fill the card: sums cut over the waves of a workgroup, small tiles"""
+    rt = _open.setdefault(name, A.AceHip(*args))
+    a = MiddleAttn(rt, 2, [0, 1], *sizes, kind=kind)
+    a.scores()
+    a.scores(causal=False)
+    a.out()
+    a.out(causal=False)
+    a.out(state=False, factor=False)
+    a.state()
+    a.state(kept=False)
     a.state(in_place=True)
     a.free()
 
