@@ -413,9 +413,20 @@ static void launch_mfma(const DevCtx& c, const LinearArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((linear_i8_mfma_kernel<MT, WJ, WN, false>), grid, block, 0, s, c, a, j_blocks, log_blocks, tiles);
 }
 
-// Outputs whose packed weights fit the workspace at a time (all of them unless the layer is large); 0: the weights are read as they lie
+// Outputs of a workgroup.  Waves along the outputs first, then along the columns: a thread then stages one or two column blocks, and what it holds of the
+// inputs in flight stays in registers (four blocks, <4, 1, 4> for 33 .. 64 outputs, spill: 141 -> 48 at N = 16384 237 us in place of 81; 141 -> 20 by
+// <2, 1, 4> 80 in place of 58).  Above 128 outputs three or four tiles a wave, whichever leaves fewer idle: 333 -> 300 at 2048 64 us by three, 76 by
+// four.  Two for all widths read the inputs more often (768 -> 2304: 2.0 ms), five do not fit the registers.
+static u32 linear_width(u32 n_out) {
+  return n_out <= 32 ? 32 : n_out <= 64 ? 64 : n_out <= 128 ? 128 : n_out <= 192 * ((n_out + 255) / 256) ? 192 : 256;
+}
+// Outputs whose packed weights fit the workspace at a time (all of them unless the layer is large); 0: the weights are read as they lie, also where
+// every workgroup has a place at once (two on each of 256 CUs) and packing is one launch more: 700 -> 1000 at N = 1024 22 us, 32 packed; 92 -> 103 at 2048,
+// two limbs, 8.7 and 11.1; at twice as many workgroups 17 -> 244 at 2048, two rows and limbs: 22.7 and 20.3
 u32 linear_pack_outputs(const DevCtx& c, const LinearArgs& a, size_t ws_bytes) {
   if (!linear_fits(c, a) || a.n_out <= 32) return 0;
+  const u32 width = linear_width(a.n_out), columns = width == 64 ? 32 : 16;
+  if ((u64)a.rows * a.n_comp * a.n_limbs * c.nrep * (c.N / columns) * ((a.n_out + width - 1) / width) <= 512) return 0;
   const u64 tile = (u64)((a.n_in + 63) / 64) * 1024, tiles = std::min(ws_bytes, (size_t)1 << 31) / tile;  // (32-bit offsets)
   if (tiles * 16 >= a.n_out) return a.n_out;
   return (u32)(tiles / 16 * 256);  // whole workgroups
@@ -429,20 +440,14 @@ void launch_linear_i8(const DevCtx& c, const LinearArgs& a, hipStream_t s) {
   if (!linear_fits(c, a)) {
     const u32 n_blocks = (c.N + 255) / 256, j_blocks = (a.n_out + kJ - 1) / kJ;
     hipLaunchKernelGGL(linear_i8_kernel, dim3(n_blocks * j_blocks * a.n_comp * a.rows, a.n_limbs, c.nrep), dim3(256), 0, s, c, a, n_blocks, j_blocks);
-  // Waves along the outputs first, then along the columns: a thread then stages one or two column blocks, and what it holds of the inputs in flight
-  // stays in registers (four blocks, <4, 1, 4> for 33 .. 64 outputs, spill: 141 -> 48 at N = 16384 237 us in place of 81; 141 -> 20 by <2, 1, 4> 80
-  // in place of 58).  Above 128 outputs three or four tiles a wave, whichever leaves fewer idle: 333 -> 300 at 2048 64 us by three, 76 by four.
-  // Two for all widths read the inputs more often (768 -> 2304: 2.0 ms), five do not fit the registers.
-  } else if (a.n_out <= 32) {
-    launch_mfma<1, 2, 2>(c, a, s);
-  } else if (a.n_out <= 64) {
-    launch_mfma<2, 2, 2>(c, a, s);
-  } else if (a.n_out <= 128) {
-    launch_mfma<2, 4, 1>(c, a, s);
-  } else if (a.n_out <= 192 * ((a.n_out + 255) / 256)) {
-    launch_mfma<3, 4, 1>(c, a, s);
-  } else {
-    launch_mfma<4, 4, 1>(c, a, s);
+    return;
+  }
+  switch (linear_width(a.n_out)) {
+    case 32: return launch_mfma<1, 2, 2>(c, a, s);
+    case 64: return launch_mfma<2, 2, 2>(c, a, s);
+    case 128: return launch_mfma<2, 4, 1>(c, a, s);
+    case 192: return launch_mfma<3, 4, 1>(c, a, s);
+    default: return launch_mfma<4, 4, 1>(c, a, s);
   }
 }
 

@@ -364,7 +364,7 @@ typedef struct acehip_mat {
  *   out[r][j] = tok[r] (*) mul[j] * sum_{i < n_in} w[j][i] in[r][i]      for each of the n_comp polynomials of the ciphertexts
  * in: rows x n_in, out: rows x n_out (head_stride unused).  d_w: [n_out][ld_w] bytes, ld_w >= n_in, no alignment asked.  d_mul: [n_out] or NULL.
  * d_tok: plaintext polynomial of row r (encoded scales of its tokens: 0 / 1 masks padding) at d_tok + r*tok_stride, or NULL.
- * The weights of more than 32 outputs are laid out in the context's workspace on `stream`: like the pipelines that keep scratch there, calls on
+ * The weights of more than 32 outputs may be laid out in the context's workspace on `stream`: like the pipelines that keep scratch there, calls on
  * one context follow each other, on one stream or ordered between streams, and graphs captured from them are not replayed at the same time. */
 #define ACEHIP_LINEAR_MAX_IN 65536
 int acehip_linear_i8(acehip_ctx* ctx, const acehip_mat* out, const acehip_mat* in, const int8_t* d_w, size_t ld_w, uint32_t rows, uint32_t n_in,

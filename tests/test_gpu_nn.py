@@ -251,6 +251,14 @@ def test_linear_shared_inputs(contexts, same, n_in, n_out):
         b.free()
 
 
+@pytest.mark.parametrize("n_out", [512, 600, 1030])
+def test_linear_weights_in_parts(contexts, n_out):
+    """as many packed weights as the workspace holds (512 outputs), or more"""
+    rt = contexts("n64")
+    assert 32 * 1024 <= rt.lib.acehip_workspace_words(rt.h) * 8 < 38 * 1024
+    linear_case(rt, 2, [0, 1], 12, 3, n_out, 3, mul=True)
+
+
 def test_linear_empty_sum_is_zero(contexts):
     linear_case(contexts("n64"), 2, [0, 1], 1, 0, 5, 2, True, True)
 
