@@ -82,7 +82,7 @@ struct Columns {
   u32 log_blocks;      // column blocks of a polynomial
 };
 
-template <int NP, int MT, int WJ, int WN, bool PACKED>
+template <int NP, int MT, int WJ, int WN, bool PACKED, bool ODD>
 __device__ __forceinline__ void linear_tiles(const DevCtx& c, const LinearArgs& a, v4i_t* frag, ulong2* factor, const DevPrime& P, u32 rep, u32 pos, const Columns& cols,
                                              u32 j0) {
   constexpr int G = 4 / WJ;  // column blocks of 16 that a thread stages
@@ -134,7 +134,7 @@ __device__ __forceinline__ void linear_tiles(const DevCtx& c, const LinearArgs& 
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int u = 0; u < G; ++u) r.v[u][i] = __builtin_bit_cast(u64, __builtin_amdgcn_raw_buffer_load_b64(d, (int)x_at[i] + u * (WN / G * 128), 0, 0));
-    const bool wrap = x_step == (last | 1u);
+    const bool wrap = x_step == (ODD ? last : last | 1u);
     x_step = wrap ? 0 : x_step + 1;
     x_tile += wrap;
     x_rest = wrap ? (x_tile < cols.n ? x_all : 0) : x_rest - 64;
@@ -282,19 +282,22 @@ __device__ __forceinline__ void linear_tiles(const DevCtx& c, const LinearArgs& 
   };
 
   // ---- the steps of all tiles in one pipeline: inputs are requested three steps ahead and staged one ahead, across the tiles' borders, so that
-  // a tile's first inputs are under way while the one before it is reduced.  Steps go in pairs (the second of the last pair may be empty).  Behind
-  // the last step weights are read again and inputs as zeros, never to be used: without a branch around the requests the compiler counts them
-  // exactly and waits for the oldest only.
+  // a tile's first inputs are under way while the one before it is reduced.  Steps go in pairs (registers and buffers in turn); ODD, an odd number of
+  // steps: so do tiles (an empty step in place of that: 14 -> 11 at N = 32768, three limbs, 37 us, 30 in pairs of tiles; 180 -> 128 at 16384 57 and
+  // 53).  Behind the last step weights are read again and inputs as zeros, never to be used: without a branch around the requests the compiler counts
+  // them exactly and waits for the oldest only.
   v4i_t *buf0 = frag, *buf1 = frag + WN * NP * 64;
   Raw raw0, raw1;
   v4i_t aw0[MT], aw1[MT];
   load_x(raw0);
+  if (ODD) x_next = block(x_tile + 1, a.in, x_base, any_row, any_off) + k_wave * xs;  // (a tile of one step)
   load_x(raw1);
+  if (ODD) x_next = block(x_tile + 1, a.in, x_base, any_row, any_off) + k_wave * xs;
   if (!PACKED && last == 0) load_w_last(0, aw0);
   else                      load_w(0, aw0);
   stage(raw0, buf0);
   load_x(raw0);
-  auto step = [&](u32 ahead, bool full, const v4i_t* buf, const v4i_t (&aw)[MT], Raw& raw, v4i_t* buf_next, v4i_t (&aw_next)[MT]) {
+  auto step = [&](u32 ahead, const v4i_t* buf, const v4i_t (&aw)[MT], Raw& raw, v4i_t* buf_next, v4i_t (&aw_next)[MT]) {
     v4i_t b[AHEAD];
     lds_barrier();
     fragments(buf, b);
@@ -303,20 +306,42 @@ __device__ __forceinline__ void linear_tiles(const DevCtx& c, const LinearArgs& 
     __builtin_amdgcn_sched_barrier(0);  // (weights first: the next step waits for them and not for the inputs behind them)
     stage(raw, buf_next);
     load_x(raw);
-    if (full) multiply(aw, buf, b);
+    multiply(aw, buf, b);
   };
-  for (tile = 0; tile < cols.n; ++tile) {
-    begin();
-    for (u32 s = 0; s <= last; s += 2) {
-      step(min(s + 1, last), true, buf0, aw0, raw1, buf1, aw1);
-      step(s + 2 > last ? 0 : s + 2, s + 1 <= last, buf1, aw1, raw0, buf0, aw0);
+  auto even = [&](u32 ahead) { step(ahead, buf0, aw0, raw1, buf1, aw1); };
+  auto odd = [&](u32 ahead) { step(ahead, buf1, aw1, raw0, buf0, aw0); };
+  if (!ODD) {
+    for (tile = 0; tile < cols.n; ++tile) {
+      begin();
+      for (u32 s = 0; s < last; s += 2) {
+        even(s + 1);
+        odd(s + 2 > last ? 0 : s + 2);
+      }
+      store();
     }
-    store();
+  } else {
+    for (tile = 0; tile < cols.n; ++tile) {
+      begin();
+      for (u32 s = 0; s < last; s += 2) {
+        even(s + 1);
+        odd(s + 2);
+      }
+      even(0);
+      store();
+      if (++tile == cols.n) break;
+      begin();
+      for (u32 s = 0; s < last; s += 2) {
+        odd(s + 1);
+        even(s + 2);
+      }
+      odd(0);
+      store();
+    }
   }
 }
 
 // A workgroup takes `tiles` column blocks one after the other; the rest of them go by launch_mfma's order.
-template <int MT, int WJ, int WN, bool PACKED>
+template <int MT, int WJ, int WN, bool PACKED, bool ODD>
 __global__ __launch_bounds__(64 * WJ * WN, 2) void linear_i8_mfma_kernel(DevCtx c, LinearArgs a, u32 j_blocks, u32 log_blocks, u32 tiles) {
   __shared__ v4i_t frag[2 * WN * 8 * 64];
   __shared__ ulong2 factor[16 * MT * WJ];
@@ -339,8 +364,8 @@ __global__ __launch_bounds__(64 * WJ * WN, 2) void linear_i8_mfma_kernel(DevCtx 
   const u32 all = (a.rows * a.n_comp) << log_blocks;
   const Columns cols{g * tiles, 1, min(tiles, all - g * tiles), log_blocks};
   const u32 j0 = jb * (16 * MT * WJ);
-  if (P.q <= kBytes7) linear_tiles<7, MT, WJ, WN, PACKED>(c, a, frag, factor, P, rep, pos, cols, j0);
-  else                linear_tiles<8, MT, WJ, WN, PACKED>(c, a, frag, factor, P, rep, pos, cols, j0);
+  if (P.q <= kBytes7) linear_tiles<7, MT, WJ, WN, PACKED, ODD>(c, a, frag, factor, P, rep, pos, cols, j0);
+  else                linear_tiles<8, MT, WJ, WN, PACKED, ODD>(c, a, frag, factor, P, rep, pos, cols, j0);
 }
 
 // What the matrix-core form does not take (linear_fits: rings below 64, primes below 2^40, inputs that share words or lie 128 MiB apart): one
@@ -404,13 +429,12 @@ static void launch_mfma(const DevCtx& c, const LinearArgs& a, hipStream_t s) {
   u32 tiles = 1;
   while (tiles < 8 && blocks / (2 * tiles) >= 1024) tiles *= 2;
   const dim3 grid((all + tiles - 1) / tiles * j_blocks, a.n_limbs, c.nrep), block(64 * WJ * WN);
+  const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, c, a, j_blocks, log_blocks, tiles); };
+  const bool odd = (a.n_in + 63) / 64 % 2 != 0;
   if constexpr (MT * WJ > 2) {  // (linear_pack_outputs)
-    if (a.packed) {
-      hipLaunchKernelGGL((linear_i8_mfma_kernel<MT, WJ, WN, true>), grid, block, 0, s, c, a, j_blocks, log_blocks, tiles);
-      return;
-    }
+    if (a.packed) return odd ? launch(linear_i8_mfma_kernel<MT, WJ, WN, true, true>) : launch(linear_i8_mfma_kernel<MT, WJ, WN, true, false>);
   }
-  hipLaunchKernelGGL((linear_i8_mfma_kernel<MT, WJ, WN, false>), grid, block, 0, s, c, a, j_blocks, log_blocks, tiles);
+  odd ? launch(linear_i8_mfma_kernel<MT, WJ, WN, false, true>) : launch(linear_i8_mfma_kernel<MT, WJ, WN, false, false>);
 }
 
 // Outputs of a workgroup.  Waves along the outputs first, then along the columns: a thread then stages one or two column blocks, and what it holds of the
