@@ -446,11 +446,14 @@ static u32 linear_width(u32 n_out) {
 }
 // Outputs whose packed weights fit the workspace at a time (all of them unless the layer is large); 0: the weights are read as they lie, also where
 // every workgroup has a place at once (two on each of 256 CUs) and packing is one launch more: 700 -> 1000 at N = 1024 22 us, 32 packed; 92 -> 103 at 2048,
-// two limbs, 8.7 and 11.1; at twice as many workgroups 17 -> 244 at 2048, two rows and limbs: 22.7 and 20.3
+// two limbs, 8.7 and 11.1; at twice as many workgroups 17 -> 244 at 2048, two rows and limbs: 22.7 and 20.3.  Rows that do not lie on words of four bytes
+// cost more each time they are read: 1151 -> 211 at 1024, two rows, 39 us, 22 packed (1148 inputs: 21 and 21); 301 -> 250 at 2048 16.3 and 13.7; few
+// inputs are worth no launch then either (151 -> 50 at 1024: 8.6 and 11.2)
 u32 linear_pack_outputs(const DevCtx& c, const LinearArgs& a, size_t ws_bytes) {
   if (!linear_fits(c, a) || a.n_out <= 32) return 0;
   const u32 width = linear_width(a.n_out), columns = width == 64 ? 32 : 16;
-  if ((u64)a.rows * a.n_comp * a.n_limbs * c.nrep * (c.N / columns) * ((a.n_out + width - 1) / width) <= 512) return 0;
+  const bool words = (((u64)(uintptr_t)a.w | a.ld_w) & 3) == 0;
+  if ((words || a.n_in <= 256) && (u64)a.rows * a.n_comp * a.n_limbs * c.nrep * (c.N / columns) * ((a.n_out + width - 1) / width) <= 512) return 0;
   const u64 tile = (u64)((a.n_in + 63) / 64) * 1024, tiles = std::min(ws_bytes, (size_t)1 << 31) / tile;  // (32-bit offsets)
   if (tiles * 16 >= a.n_out) return a.n_out;
   return (u32)(tiles / 16 * 256);  // whole workgroups
