@@ -553,20 +553,21 @@ static void launch_shared(const DevCtx& c, const LinattnArgs& a, hipStream_t s) 
 
 // Where a workgroup for each result leaves every workgroup a place (eight on each of 256 CUs), the sums are cut over its waves: 4 x 4 scores of 64 features
 // at N = 1024 8.3 us, 21 by the next form; a 64 x 64 state read by one token 15 and 25; with more of them it loses (16 x 16 states, 16 tokens: 24 us, 20).
-// Launches that leave half the places of the larger form empty take one result a wave and two terms a stage (9 x 9 scores of 51 features at 2048: 25 us, 38
-// by 2 x 2; from 512 workgroups on it loses: 8 x 8 scores of 24 features at 4096: 27 us, 24).
-// One row: its operands are read once whatever the form, and waiting for each other costs (48 x 48 state at N = 8192: 0.72 ms, 0.86 shared).  Two rows or
-// more share (2 x 40 x 4 scores at 8192: 53 us, 91 unshared by tiles of 4 x 8; 64 x 2 state of four tokens 0.55 ms, 1.09).
+// Tiles of 2 x 2 results, two terms a stage, where their workgroups have a place at once (four on each CU; 9 x 9 scores of 51 features at 2048: 25 us, 38 by
+// 4 x 4; with 1280 workgroups, 8 x 8 scores of 24 features at 4096, 27 and 24), or where 4 x 4 leave more idle than they save: one takes as long as 2.15
+// of 2 x 2 (2 x 2 scores of 40 features, eight heads, three limbs at 8192: 100 us, 124 by 4 x 4; 6 x 6 states, 20 tokens: 359 and 336).
+// One row: its operands are read once whatever the form, and waiting for each other costs (48 x 48 state at N = 8192: 0.72 ms, 0.86 shared) unless half the
+// places stay empty (48 x 48 at 1024, three limbs: 31 us, 27 shared).  Two rows or more share (2 x 40 x 4 scores at 8192: 53 us, 91 unshared by tiles of
+// 4 x 8; 64 x 2 state of four tokens 0.55 ms, 1.09).
 void launch_linattn(const DevCtx& c, const LinattnArgs& a, hipStream_t s) {
   const bool row = a.M == 1;
-  const u64 blocks = (u64)((c.N + 63) / 64) * a.n_heads * a.n_limbs * c.nrep;
-  const u32 m = row ? 1 : 4, n = row ? 16 : 4;  // results of a workgroup of the larger forms
-  const u64 groups = blocks * ((a.M + m - 1) / m) * ((a.Nn + n - 1) / n);
-  if (!a.wide_primes)                                                         launch_rows<1, 1, 1, false>(c, a, s);
-  else if (blocks * a.M * a.Nn <= 2048 && (u64)a.t1.K + a.t2.K >= 16)         launch_rows<1, 1, 4, true>(c, a, s);
-  else if (c.N >= 64 && groups < 512)                                         launch_shared<1, 1, 2, 2, 2, 4>(c, a, s);
-  else if (c.N >= 64 && !row)                                                 launch_shared<2, 2, 2, 2, 1, 4>(c, a, s);
-  else                                                                        launch_rows<4, 4, 1, true>(c, a, s);
+  const u64 blocks = (u64)((c.N + 63) / 64) * a.n_heads * a.n_limbs * c.nrep, small = Tiles(a, 2, 2).all, large = Tiles(a, 4, 4).all;
+  const bool spare = row ? blocks * ((a.Nn + 15) / 16) < 512 : blocks * small <= 1024 || small * 20 < large * 43;
+  if (!a.wide_primes)                                                 launch_rows<1, 1, 1, false>(c, a, s);
+  else if (blocks * a.M * a.Nn <= 2048 && (u64)a.t1.K + a.t2.K >= 16) launch_rows<1, 1, 4, true>(c, a, s);
+  else if (c.N >= 64 && spare)                                        launch_shared<1, 1, 2, 2, 2, 4>(c, a, s);
+  else if (c.N >= 64 && !row)                                         launch_shared<2, 2, 2, 2, 1, 4>(c, a, s);
+  else                                                                launch_rows<4, 4, 1, true>(c, a, s);
 }
 
 }  // namespace acehip
