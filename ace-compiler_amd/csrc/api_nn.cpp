@@ -171,18 +171,8 @@ int acehip_linear_i8(acehip_ctx* c, const acehip_mat* out, const acehip_mat* in,
   a.wide_primes = k.primes_above(40);
   // (weights inside the arena differ from replica to replica: they are read as they lie)
   const bool shared = c->dc.rep_span == 0 || (u64)(uintptr_t)d_w - c->dc.rep_lo >= c->dc.rep_span;
-  const u32 part = shared ? linear_pack_outputs(c->dc, a, c->ws_words * sizeof(u64)) : 0;
-  for (u32 j = 0; j < n_out; j += part ? part : n_out) {
-    a.out.d = y.m.d + (u64)j * y.m.col;
-    a.w = d_w + (u64)j * ld_w;
-    a.mul = d_mul ? d_mul + j : nullptr;
-    a.n_out = part ? std::min(part, n_out - j) : n_out;
-    if (part) {
-      launch_linear_pack(a, c->ws, (hipStream_t)s);
-      a.packed = c->ws;
-    }
-    for (const DevCtx& dc : launch_dcs(c)) launch_linear_i8(dc, a, (hipStream_t)s);
-  }
+  const DcList l = launch_dcs(c);
+  launch_linear(c->dc, l.d, l.n, a, shared ? c->ws : nullptr, c->ws_words * sizeof(u64), (hipStream_t)s);
   const u64 limb = 8ull * c->hp.N * n_limbs * rows;
   stat(ST_LINEAR, (u64)rows * n_out, limb * ((u64)n_comp * n_in + (u64)n_comp * n_out + (d_tok ? 1 : 0)) + (u64)n_in * n_out);
   return post_launch();

@@ -51,6 +51,12 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// The first of 16 bytes that hold the weights from byte `at` of the array on, as far as they are there; of an array of 16 bytes at least.
+__host__ __device__ __forceinline__ u64 linear_pack_from(u64 at, u32 n_out, u64 ld_w, u32 n_in) {
+  const u64 last = (n_out - 1) * ld_w + n_in - 16;
+  return at < last ? at : last;
+}
+
 // Weights as A fragments, [tile of 16 outputs][step][lane] of 16 bytes, zero past the matrix.  In memory a fragment's lanes read 16 bytes from each of
 // 16 rows, which costs the L1 cache 64 look-ups (four waves a fragment long: the product waits for them); packed, a fragment is 1 KiB in a row:
 // 2.62 -> 1.91 ms (768 -> 2304 at N = 16384), with the launch.  Up to 32 outputs one wave reads each fragment and the launch costs what it saves
@@ -59,10 +65,10 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const int8_t* w, u64 l
   const u32 f = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63u;
   if (f >= n_frags) return;
   const u32 j = (f / steps) * 16 + (lane & 15u), k = (f % steps) * 64 + 16 * (lane >> 4);
-  // 16 bytes from the array, the last ones of it at most (linear_fits: it has 16), moved to their place; those past the row are cleared
+  // 16 bytes from the array, the last ones of it at most (linear_fits asks for 16 of every part), moved to their place; those past the row are cleared
   unsigned __int128 v = 0;
   if (j < n_out && k < n_in) {
-    const u64 at = j * ld_w + k, last = (n_out - 1) * ld_w + n_in - 16, from = min(at, last);
+    const u64 at = j * ld_w + k, from = linear_pack_from(at, n_out, ld_w, n_in);
     v = __builtin_bit_cast(unsigned __int128, (v4i_t) * (const GLOBAL v4i_any_t*)(global(w) + from)) >> (8 * (u32)(at - from));
     if (n_in - k < 16) v &= ((unsigned __int128)1 << (8 * (n_in - k))) - 1;
   }
@@ -449,8 +455,9 @@ static u32 linear_width(u32 n_out) {
 // two limbs, 8.7 and 11.1; at twice as many workgroups 17 -> 244 at 2048, two rows and limbs: 22.7 and 20.3.  Rows that do not lie on words of four bytes
 // cost more each time they are read: 1151 -> 211 at 1024, two rows, 39 us, 22 packed (1148 inputs: 21 and 21); 301 -> 250 at 2048 16.3 and 13.7; few
 // inputs are worth no launch then either (151 -> 50 at 1024: 8.6 and 11.2)
-u32 linear_pack_outputs(const DevCtx& c, const LinearArgs& a, size_t ws_bytes) {
-  if (!linear_fits(c, a) || a.n_out <= 32) return 0;
+static bool linear_takes_packed(const DevCtx& c, const LinearArgs& a) { return linear_fits(c, a) && a.n_out > 32; }
+static u32 linear_pack_outputs(const DevCtx& c, const LinearArgs& a, size_t ws_bytes) {
+  if (!linear_takes_packed(c, a)) return 0;
   const u32 width = linear_width(a.n_out), columns = width == 64 ? 32 : 16;
   const bool words = (((u64)(uintptr_t)a.w | a.ld_w) & 3) == 0;
   if ((words || a.n_in <= 256) && (u64)a.rows * a.n_comp * a.n_limbs * c.nrep * (c.N / columns) * ((a.n_out + width - 1) / width) <= 512) return 0;
@@ -458,12 +465,12 @@ u32 linear_pack_outputs(const DevCtx& c, const LinearArgs& a, size_t ws_bytes) {
   if (tiles * 16 >= a.n_out) return a.n_out;
   return (u32)(tiles / 16 * 256);  // whole workgroups
 }
-void launch_linear_pack(const LinearArgs& a, void* out, hipStream_t s) {
+static void launch_linear_pack(const LinearArgs& a, void* out, hipStream_t s) {
   const u32 steps = (a.n_in + 63) / 64, n_frags = (a.n_out + 15) / 16 * steps;
   hipLaunchKernelGGL(linear_pack_kernel, dim3((n_frags + 3) / 4), dim3(256), 0, s, a.w, a.ld_w, a.n_in, a.n_out, steps, n_frags, (v4i_t*)out);
 }
 
-void launch_linear_i8(const DevCtx& c, const LinearArgs& a, hipStream_t s) {
+static void launch_linear_i8(const DevCtx& c, const LinearArgs& a, hipStream_t s) {
   if (!linear_fits(c, a)) {
     const u32 n_blocks = (c.N + 255) / 256, j_blocks = (a.n_out + kJ - 1) / kJ;
     hipLaunchKernelGGL(linear_i8_kernel, dim3(n_blocks * j_blocks * a.n_comp * a.rows, a.n_limbs, c.nrep), dim3(256), 0, s, c, a, n_blocks, j_blocks);
@@ -475,6 +482,21 @@ void launch_linear_i8(const DevCtx& c, const LinearArgs& a, hipStream_t s) {
     case 128: return launch_mfma<2, 4, 1>(c, a, s);
     case 192: return launch_mfma<3, 4, 1>(c, a, s);
     default: return launch_mfma<4, 4, 1>(c, a, s);
+  }
+}
+
+// A last part may be one that the packed form does not take: up to 32 outputs, or weights of fewer bytes than a fragment's 16.
+void launch_linear(const DevCtx& c, const DevCtx* launches, u32 n_launches, LinearArgs a, void* ws, size_t ws_bytes, hipStream_t s) {
+  const LinearArgs all = a;
+  const u32 part = ws ? linear_pack_outputs(c, a, ws_bytes) : 0;
+  for (u32 j = 0; j < all.n_out; j += part ? part : all.n_out) {
+    a.out.d = all.out.d + (u64)j * all.out.col;
+    a.w = all.w + (u64)j * all.ld_w;
+    a.mul = all.mul ? all.mul + j : nullptr;
+    a.n_out = part ? std::min(part, all.n_out - j) : all.n_out;
+    a.packed = part && linear_takes_packed(c, a) ? ws : nullptr;
+    if (a.packed) launch_linear_pack(a, ws, s);
+    for (u32 l = 0; l < n_launches; ++l) launch_linear_i8(launches[l], a, s);
   }
 }
 

@@ -29,11 +29,10 @@ struct LinearArgs {
   u64 tok_stride;
   u32 rows, n_in, n_out, n_comp, level, pos0, n_limbs;
   bool wide_primes;    // every prime of the call is above 2^40
-  const void* packed = nullptr;  // the weights as launch_linear_pack left them
+  const void* packed = nullptr;  // the weights as linear_pack_kernel left them
 };
-u32 linear_pack_outputs(const DevCtx& c, const LinearArgs& a, size_t ws_bytes);
-void launch_linear_pack(const LinearArgs& a, void* out, hipStream_t s);
-void launch_linear_i8(const DevCtx& c, const LinearArgs& a, hipStream_t s);
+// on every one of the launch sets; ws: memory for packed weights, or null: they are read as they lie
+void launch_linear(const DevCtx& c, const DevCtx* launches, u32 n_launches, LinearArgs a, void* ws, size_t ws_bytes, hipStream_t s);
 
 // cos and sin of pos[axis[i]][t] * freq[i] (rope.hip)
 constexpr u32 ROPE_PAIRS_MAX = 256;  // pairs per launch: a kernel argument
