@@ -13,7 +13,7 @@ struct View {
   u64 n[4];  // heads, rows, cols, comps
   u64 lo = 0, hi = 0;  // byte addresses of its first word and behind its last (the limbs of the call)
   u64 limb0 = 0, span = 0;  // bytes from a polynomial's start to the first limb, bytes of the limbs
-  bool empty() const { return n[0] * n[1] * n[2] * n[3] == 0 || span == 0; }
+  bool empty() const { return n[0] == 0 || n[1] == 0 || n[2] == 0 || n[3] == 0 || span == 0; }
   u64 stride(int k) const { return k == 0 ? m.head : k == 1 ? m.row : k == 2 ? m.col : m.comp; }
 };
 
@@ -77,7 +77,12 @@ bool starts(const View& v, std::vector<u64>& s) try {
 } catch (const std::bad_alloc&) {
   return false;
 }
-u64 count(const View& v) { return v.n[0] * v.n[1] * v.n[2] * v.n[3]; }
+// polynomials of a matrix (its counts are not 0), 2^64 - 1 where there are more
+u64 count(const View& v) {
+  u64 c = 1;
+  for (u64 n : v.n) c = c > ~0ull / n ? ~0ull : c * n;
+  return c;
+}
 
 // every polynomial of a result has words of its own
 int check_result(const Call& k, const View& v) {
