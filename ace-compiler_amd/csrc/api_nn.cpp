@@ -161,7 +161,7 @@ int acehip_linear_i8(acehip_ctx* c, const acehip_mat* out, const acehip_mat* in,
   if (int e = check_array(k, y, d_mul, (i128)8 * n_out, 8)) return e;
   if (int e = check_array(k, y, d_tok, (i128)8 * (rows - 1) * tok_stride + y.limb0 + y.span, 8)) return e;
   const i128 polys = (i128)rows * n_comp;
-  if (int e = check_blocks(k, polys * ((c->hp.N + 255) / 256) * ((n_out + 7) / 8))) return e;
+  if (int e = check_blocks(k, polys * ((c->hp.N + 255) / 256) * (((u64)n_out + 7) / 8))) return e;
   if (int e = check_dev(c)) return e;
   LinearArgs a;
   a.out = y.m;

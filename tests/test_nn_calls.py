@@ -25,3 +25,9 @@ def test_counts_past_64_bits(rt, n):  # noqa: F811
             c.a["w"] = 1
         assert c.call(rt) == EINVAL, c
         assert "too many" in rt.err() or "overlap" in rt.err(), rt.err()
+
+
+@pytest.mark.parametrize("n_out", [(1 << 32) - 7, (1 << 32) - 1, 1 << 31])
+def test_linear_outputs_near_32_bits(rt, n_out):  # noqa: F811
+    c = changed(Linear, out=Mat(1 << 45, 0, 0, 192, 0), rows=1, comps=1, n_out=n_out, ld=7, w=1 << 61, mul=None, tok=None)
+    assert c.call(rt) == EINVAL and "too many" in rt.err()
