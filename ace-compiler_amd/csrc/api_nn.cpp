@@ -11,7 +11,7 @@ using i128 = __int128;
 struct View {
   CtMat m;
   u64 n[4];  // heads, rows, cols, comps
-  u64 lo = 0, hi = 0;  // byte addresses of its first word and behind its last (the limbs of the call)
+  u64 lo = 0, hi = 0;  // byte addresses of its first word and behind its last one (the limbs of the call)
   u64 limb0 = 0, span = 0;  // bytes from a polynomial's start to the first limb, bytes of the limbs
   bool empty() const { return n[0] == 0 || n[1] == 0 || n[2] == 0 || n[3] == 0 || span == 0; }
   u64 stride(int k) const { return k == 0 ? m.head : k == 1 ? m.row : k == 2 ? m.col : m.comp; }
@@ -66,64 +66,129 @@ struct Call {
   }
 };
 
-constexpr u64 kListed = 1ull << 20;  // polynomials that are listed one by one where bounds alone do not tell
-bool starts(const View& v, std::vector<u64>& s) try {
-  for (u64 h = 0; h < v.n[0]; ++h)
-    for (u64 r = 0; r < v.n[1]; ++r)
-      for (u64 k = 0; k < v.n[2]; ++k)
-        for (u64 p = 0; p < v.n[3]; ++p) s.push_back(v.lo + 8 * (h * v.m.head + r * v.m.row + k * v.m.col + p * v.m.comp));
+// Ranges of bytes [lo + sum_k i_k stride_k, .. + span), 0 <= i_k < n_k: the polynomials of a matrix (the limbs of the call), the rows of a table.
+struct Ranges {
+  u64 lo, span, stride[4] = {}, n[4] = {1, 1, 1, 1};
+};
+Ranges ranges(const View& v) {
+  Ranges r{v.lo, v.span};
+  for (int k = 0; k < 4; ++k) r.stride[k] = 8 * v.stride(k), r.n[k] = v.n[k];
+  return r;
+}
+// Whether two ranges of two sets meet (or two of one set), by the differences of their starts, d + sum_k c_k stride_k: the axes are gone through from
+// the widest stride on, and of each only the c_k are followed with which the axes behind it can still bring the difference near zero -- a few of them
+// where the strides are nested (two interleaved matrices of 2^19 polynomials: 3 us a call in place of 42 ms, listed and sorted).
+enum Meet { APART, MEET, UNKNOWN };
+class Differences {
+  struct Axis {
+    i128 stride, lo, hi;
+  };
+  Axis axis_[8];
+  int n_ = 0;
+  i128 below_[9], above_[9];  // what the axes from k on add
+  i128 from_, to_;            // of ranges that meet: from < difference < to
+  u32 steps_ = 0;
+
+ public:
+  static constexpr u32 kSteps = 1u << 14;  // (some milliseconds)
+  Differences(i128 from, i128 to) : from_(from), to_(to) {}
+  // c in [lo, hi]; false: there was an axis of this stride
+  bool axis(u64 stride, i128 lo, i128 hi) {
+    for (int k = 0; k < n_; ++k)
+      if (axis_[k].stride == (i128)stride) {
+        axis_[k].lo += lo;
+        axis_[k].hi += hi;
+        return false;
+      }
+    axis_[n_++] = Axis{(i128)stride, lo, hi};
+    return true;
+  }
+  // but_zero: the difference of all c = 0 does not count
+  Meet find(i128 d, bool but_zero) {
+    std::sort(axis_, axis_ + n_, [](const Axis& x, const Axis& y) { return x.stride > y.stride; });
+    below_[n_] = above_[n_] = 0;
+    for (int k = n_ - 1; k >= 0; --k) {
+      below_[k] = below_[k + 1] + axis_[k].lo * axis_[k].stride;
+      above_[k] = above_[k + 1] + axis_[k].hi * axis_[k].stride;
+    }
+    return step(0, d, but_zero);
+  }
+
+ private:
+  static i128 floor_div(i128 a, i128 b) { return a / b - (a % b < 0); }
+  Meet step(int k, i128 d, bool zero) {
+    if (k == n_) return zero || d <= from_ || d >= to_ ? APART : MEET;
+    if (++steps_ > kSteps) return UNKNOWN;
+    const Axis& a = axis_[k];
+    const i128 lo = std::max(a.lo, floor_div(from_ - above_[k + 1] - d, a.stride) + 1), hi = std::min(a.hi, -floor_div(d + below_[k + 1] - to_, a.stride) - 1);
+    for (i128 c = lo; c <= hi; ++c)
+      if (const Meet m = step(k + 1, d + c * a.stride, zero && c == 0)) return m;
+    return APART;
+  }
+};
+
+// Strides that cross too often for that: the ranges one by one.
+constexpr u64 kListed = 1ull << 20;
+u64 count(const Ranges& r) {  // (no n is 0; 2^64 - 1 where there are more)
+  u64 c = 1;
+  for (u64 n : r.n) c = c > ~0ull / n ? ~0ull : c * n;
+  return c;
+}
+bool starts(const Ranges& r, std::vector<u64>& s) try {
+  if (count(r) > kListed) return false;
+  for (u64 i = 0; i < r.n[0]; ++i)
+    for (u64 j = 0; j < r.n[1]; ++j)
+      for (u64 k = 0; k < r.n[2]; ++k)
+        for (u64 l = 0; l < r.n[3]; ++l) s.push_back(r.lo + i * r.stride[0] + j * r.stride[1] + k * r.stride[2] + l * r.stride[3]);
   std::sort(s.begin(), s.end());
   return true;
 } catch (const std::bad_alloc&) {
   return false;
 }
-// polynomials of a matrix (its counts are not 0), 2^64 - 1 where there are more
-u64 count(const View& v) {
-  u64 c = 1;
-  for (u64 n : v.n) c = c > ~0ull / n ? ~0ull : c * n;
-  return c;
+bool apart(const Ranges& x) {
+  Differences d(-(i128)x.span, x.span);
+  for (int k = 0; k < 4; ++k)
+    if (x.n[k] > 1 && (x.stride[k] == 0 || !d.axis(x.stride[k], -(i128)(x.n[k] - 1), x.n[k] - 1))) return false;
+  const Meet m = d.find(0, true);
+  if (m != UNKNOWN) return m == APART;
+  std::vector<u64> s;
+  if (!starts(x, s)) return false;
+  for (size_t i = 1; i < s.size(); ++i)
+    if (s[i] - s[i - 1] < x.span) return false;
+  return true;
+}
+bool apart(const Ranges& x, const Ranges& y) {
+  Differences d(-(i128)x.span, y.span);
+  for (int k = 0; k < 4; ++k) {
+    if (x.n[k] > 1 && x.stride[k]) d.axis(x.stride[k], 0, x.n[k] - 1);
+    if (y.n[k] > 1 && y.stride[k]) d.axis(y.stride[k], -(i128)(y.n[k] - 1), 0);
+  }
+  const Meet m = d.find((i128)x.lo - y.lo, false);
+  if (m != UNKNOWN) return m == APART;
+  std::vector<u64> s, t;
+  if (!starts(x, s) || !starts(y, t)) return false;
+  for (u64 at : t) {  // the last range of x that starts up to there, and the one behind it
+    const auto it = std::upper_bound(s.begin(), s.end(), at);
+    if ((it != s.begin() && at - *(it - 1) < x.span) || (it != s.end() && *it - at < y.span)) return false;
+  }
+  return true;
 }
 
 // every polynomial of a result has words of its own
 int check_result(const Call& k, const View& v) {
   if (v.empty()) return ACEHIP_OK;
   if (int e = k.memory(v.lo, v.hi, true)) return e;
-  std::pair<u64, u64> d[4];
-  for (int i = 0; i < 4; ++i) d[i] = {v.stride(i), v.n[i]};
-  std::sort(d, d + 4);
-  u64 inner = v.span / 8;  // words of what lies inside the next stride
-  bool nested = true;
-  for (const auto& [stride, n] : d) {
-    if (n == 1) continue;
-    nested = nested && stride >= inner;
-    inner += (n - 1) * stride;
-  }
-  if (nested) return ACEHIP_OK;
-  std::vector<u64> s;
-  if (count(v) <= kListed && starts(v, s)) {
-    bool apart = true;
-    for (size_t i = 1; i < s.size(); ++i) apart = apart && s[i] - s[i - 1] >= v.span;
-    if (apart) return ACEHIP_OK;
-  }
-  return k.bad("the polynomials of a result overlap");
-}
-int check_apart(const Call& k, const View& out, u64 lo, u64 hi) {
-  if (out.empty() || lo >= out.hi || hi <= out.lo) return ACEHIP_OK;
-  return k.bad("a result overlaps an operand");
+  return apart(ranges(v)) ? ACEHIP_OK : k.bad("the polynomials of a result overlap");
 }
 int check_apart(const Call& k, const View& out, const View& in) {
-  if (out.empty() || in.empty() || in.lo >= out.hi || in.hi <= out.lo) return ACEHIP_OK;
-  std::vector<u64> s, t;
-  if (count(out) <= kListed && count(in) <= kListed && starts(out, s) && starts(in, t)) {
-    bool apart = true;
-    for (u64 x : t) {  // the first result that ends behind x's start
-      auto it = std::upper_bound(s.begin(), s.end(), x);
-      if (it != s.begin() && x - *(it - 1) < out.span) apart = false;
-      if (it != s.end() && *it - x < in.span) apart = false;
-    }
-    if (apart) return ACEHIP_OK;
-  }
-  return k.bad("a result overlaps an operand");
+  return out.empty() || in.empty() || apart(ranges(out), ranges(in)) ? ACEHIP_OK : k.bad("a result overlaps an operand");
+}
+// a table of plaintexts, of rows and of columns
+int check_table(const Call& k, const View& out, const u64* p, u64 rows, u64 row_stride, u64 cols, u64 col_stride) {
+  const acehip_mat m{const_cast<u64*>(p), 0, row_stride, col_stride, 0};
+  View t;
+  if (int e = k.view(t, &m, 1, rows, cols, 1)) return e;
+  return check_apart(k, out, t);
 }
 // a plain array argument: alignment, arena, distance from the result
 int check_array(const Call& k, const View& out, const void* p, i128 bytes, u32 align) {
@@ -132,7 +197,7 @@ int check_array(const Call& k, const View& out, const void* p, i128 bytes, u32 a
   if (at % align) return k.bad("an array is not aligned to its type");
   if (bytes > ((i128)1 << 62) || at > ~0ull - (u64)bytes) return k.bad("the strides of an array leave the address space");
   if (int e = k.memory(at, at + (u64)bytes, false)) return e;
-  return check_apart(k, out, at, at + (u64)bytes);
+  return out.empty() || apart(ranges(out), Ranges{at, (u64)bytes}) ? ACEHIP_OK : k.bad("a result overlaps an operand");
 }
 // a launch takes less than 2^32 lanes along x: workgroups of 256 there (limbs and replicas are its y and z)
 int check_blocks(const Call& k, i128 blocks) {
@@ -159,7 +224,8 @@ int acehip_linear_i8(acehip_ctx* c, const acehip_mat* out, const acehip_mat* in,
   if (n_in)
     if (int e = check_array(k, y, d_w, (i128)(n_out - 1) * ld_w + n_in, 1)) return e;
   if (int e = check_array(k, y, d_mul, (i128)8 * n_out, 8)) return e;
-  if (int e = check_array(k, y, d_tok, (i128)8 * (rows - 1) * tok_stride + y.limb0 + y.span, 8)) return e;
+  if (d_tok)
+    if (int e = check_table(k, y, d_tok, rows, tok_stride, 1, 0)) return e;
   const i128 polys = (i128)rows * n_comp;
   if (int e = check_blocks(k, polys * ((c->hp.N + 255) / 256) * (((u64)n_out + 7) / 8))) return e;
   if (int e = check_dev(c)) return e;
@@ -200,7 +266,9 @@ int acehip_rope_messages(acehip_ctx* c, double* d_cos, double* d_sin, size_t out
     if ((uintptr_t)p % 8) return k.bad("an array is not aligned to its type");
   if (out_bytes > ((i128)1 << 62) || pos_bytes > ((i128)1 << 62)) return k.bad("the strides of an array leave the address space");
   const u64 co = (u64)(uintptr_t)d_cos, si = (u64)(uintptr_t)d_sin, po = (u64)(uintptr_t)d_pos, ob = (u64)out_bytes, pb = (u64)pos_bytes;
-  if ((co < si + ob && si < co + ob) || (co < po + pb && po < co + ob) || (si < po + pb && po < si + ob)) return k.bad("a result overlaps an operand");
+  const Ranges vc{co, 8ull * n_pos, {8 * out_stride}, {n_pairs, 1, 1, 1}}, vs{si, 8ull * n_pos, {8 * out_stride}, {n_pairs, 1, 1, 1}},
+      vp{po, 8ull * n_pos, {8 * pos_stride}, {n_axes, 1, 1, 1}};
+  if (!apart(vc, vs) || !apart(vc, vp) || !apart(vs, vp)) return k.bad("a result overlaps an operand");
   // (shared by all replicas like the plaintexts made of them: the arena is for polynomials)
   for (const auto& [p, b] : {std::pair<u64, u64>{co, ob}, {si, ob}, {po, pb}})
     if (c->dc.rep_span && p < c->dc.rep_lo + c->dc.rep_span && p + b > c->dc.rep_lo) return k.bad("positions and messages do not lie in the arena");
@@ -233,9 +301,8 @@ int acehip_rope(acehip_ctx* c, const acehip_mat* out, const acehip_mat* in, cons
   const bool same = x.m.d == y.m.d && x.m.head == y.m.head && x.m.row == y.m.row && x.m.col == y.m.col && x.m.comp == y.m.comp;
   if (!same)
     if (int e = check_apart(k, y, x)) return e;
-  const i128 table = (i128)8 * (dim / 2 - 1) * pair_stride + (i128)8 * (rows - 1) * row_stride + y.limb0 + y.span;
-  if (int e = check_array(k, y, d_cos, table, 8)) return e;
-  if (int e = check_array(k, y, d_sin, table, 8)) return e;
+  for (const u64* table : {d_cos, d_sin})
+    if (int e = check_table(k, y, table, rows, row_stride, dim / 2, pair_stride)) return e;
   if (int e = check_blocks(k, (i128)((c->hp.N + 255) / 256) * (dim / 2) * rows)) return e;
   if (int e = check_dev(c)) return e;
   RopeArgs a;

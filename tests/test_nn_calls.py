@@ -1,7 +1,8 @@
 """CPU tests of the argument checks of the operators on ciphertexts (csrc/api_nn.cpp) at the calls that tests/test_nn_refusals.py leaves out: a call that
 is refused says so (ACEHIP_EINVAL), one that would run says that there is no device (ACEHIP_ENODEV)."""
+import numpy as np
 import pytest
-from test_nn_refusals import BASE, EINVAL, FAR, Linear, Out, Rope, Scores, State, changed, rt  # noqa: F401  (a fixture)
+from test_nn_refusals import BASE, EINVAL, ENODEV, FAR, POLY, Linear, Messages, Out, Rope, Scores, State, changed, rt  # noqa: F401  (a fixture)
 
 import ace_compiler_amd as A
 
@@ -31,3 +32,75 @@ def test_counts_past_64_bits(rt, n):  # noqa: F811
 def test_linear_outputs_near_32_bits(rt, n_out):  # noqa: F811
     c = changed(Linear, out=Mat(1 << 45, 0, 0, 192, 0), rows=1, comps=1, n_out=n_out, ld=7, w=1 << 61, mul=None, tok=None)
     assert c.call(rt) == EINVAL and "too many" in rt.err()
+
+
+# ---- which operands meet ---------------------------------------------------------------------------------------------------------------
+def starts(m, *n):
+    """byte addresses of a matrix's polynomials, one behind the other"""
+    s = np.array([m.data], dtype=np.int64)
+    for stride, count in zip((m.head_stride, m.row_stride, m.col_stride, m.comp_stride), n):
+        s = (s[:, None] + 8 * stride * np.arange(count)).ravel()
+    return s
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_random_layouts(rt, seed):  # noqa: F811
+    """a call is refused if and only if two polynomials of its result, or one of them and one of an operand, have a word in common"""
+    rng = np.random.default_rng(seed)
+    verdicts = [0, 0]
+    for _ in range(100):
+        rows, n_in, n_out, comps = (int(v) for v in rng.integers(1, 5, 4))
+        unit = int(rng.choice([1, 1, 2, 4]))
+        stride = lambda most: int(rng.integers(1, most)) * POLY // unit + int(rng.integers(0, 40) == 0)  # noqa: B023, E731
+        out = Mat(BASE + 8 * POLY * 40, 0, *(int(v) for v in rng.permutation([stride(30), stride(12), stride(5)])))
+        x = Mat(BASE + 8 * (POLY * int(rng.integers(0, 90)) // unit), 0, *(int(v) * (rng.random() > 0.2) for v in rng.permutation([out.row_stride, out.col_stride, stride(9)])))
+        tok = Mat(BASE + 8 * (POLY * int(rng.integers(0, 90)) // unit), 0, out.row_stride if rng.random() < 0.5 else stride(30), 0, 0)
+        y, bad = starts(out, 1, rows, n_out, comps), False
+        for other in (y, starts(x, 1, rows, n_in, comps), starts(tok, 1, rows, 1, 1)):
+            near = np.abs(other[:, None] - y[None]) < 8 * POLY
+            bad |= bool(near.sum() > len(y) if other is y else near.any())
+        c = changed(Linear, out=out, x=x, rows=rows, n_in=n_in, n_out=n_out, comps=comps, tok=tok.data, ts=tok.row_stride)
+        assert c.call(rt) == (EINVAL if bad else ENODEV), (rt.err(), c.a, [getattr(out, f) for f, _ in Mat._fields_], [getattr(x, f) for f, _ in Mat._fields_])
+        verdicts[bad] += 1
+    assert min(verdicts) >= 10
+
+
+def test_large_interleaved_operands(rt):  # noqa: F811
+    """inputs and results side by side, [row][column][input, result][polynomial], 2^22 polynomials each"""
+    rows, cols = 1 << 10, 1 << 11
+    side = dict(head_stride=0, row_stride=cols * 4 * POLY, col_stride=4 * POLY, comp_stride=POLY)
+    out, x = Mat(BASE, **side), Mat(BASE + 16 * POLY, **side)
+    c = changed(Linear, out=out, x=x, rows=rows, n_in=cols, n_out=cols, ld=cols, comps=2, w=BASE << 8, mul=None, tok=None)
+    assert c.call(rt) == ENODEV, rt.err()
+    x.data -= 8
+    assert c.call(rt) == EINVAL and "overlaps" in rt.err()
+
+
+def test_strides_that_cross(rt):  # noqa: F811
+    """too many differences to follow one by one: even places against odd ones, and against even ones"""
+    out = Mat(BASE + 8 * POLY, 0, 640 * POLY, 6 * POLY, 2 * POLY)
+    x = Mat(BASE, 0, 638 * POLY, 10 * POLY, 4 * POLY)
+    c = changed(Linear, out=out, x=x, rows=100, n_in=100, n_out=99, ld=100, comps=3, w=BASE << 8, mul=None, tok=None)
+    assert c.call(rt) == ENODEV, rt.err()
+    out.data += 8 * POLY
+    assert c.call(rt) == EINVAL and "overlaps" in rt.err()
+
+
+def test_tables_between_results(rt):  # noqa: F811
+    """a row's plaintext behind its results; cosines and sines behind the features that they turn; both messages of a pair side by side"""
+    row = 11 * POLY
+    c = changed(Linear, out=Mat(BASE, 0, row, 2 * POLY, POLY), tok=BASE + 8 * 10 * POLY, ts=row)
+    assert c.call(rt) == ENODEV, rt.err()
+    assert changed(Linear, out=Mat(BASE, 0, row, 2 * POLY, POLY), tok=BASE + 8 * 10 * POLY, ts=row - 1).call(rt) == EINVAL
+    row = (2 * 8 * 2 + 8) * POLY
+    turned = dict(out=Mat(BASE, 16 * POLY, row, 2 * POLY, POLY), c=BASE + 8 * 32 * POLY, s=BASE + 8 * 33 * POLY, ps=2 * POLY, rs=row)
+    c = changed(Rope, **turned)
+    assert c.call(rt) == ENODEV, rt.err()
+    assert changed(Rope, **{**turned, "c": turned["c"] - 8}).call(rt) == EINVAL
+    assert changed(Rope, **{**turned, "rs": row - 32 * POLY}).call(rt) == EINVAL
+    c = changed(Messages, cos=BASE, sin=BASE + 80, os=20)
+    assert c.call(rt) == ENODEV, rt.err()
+    assert changed(Messages, cos=BASE, sin=BASE + 72, os=20).call(rt) == EINVAL
+    assert changed(Messages, cos=BASE, sin=BASE + 80, os=19).call(rt) == EINVAL
+    assert changed(Messages, cos=BASE, sin=BASE + FAR, os=30, pos=BASE + 80, ps=30).call(rt) == ENODEV, rt.err()
+    assert changed(Messages, cos=BASE, sin=BASE + FAR, os=30, pos=BASE + 80, ps=10).call(rt) == EINVAL
