@@ -331,12 +331,16 @@ static u64 seen(u64 n_q, u64 n_k, int causal) {
 }
 static int run_linattn(const Call& k, LinattnArgs& a, const View& y, u64 polys, acehip_stream s) {
   acehip_ctx* c = k.c;
-  if (int e = check_blocks(k, (i128)((c->hp.N + 63) / 64) * a.Nn * a.M * a.n_heads)) return e;
-  if (int e = check_dev(c)) return e;
   a.out = y.m;
   a.level = k.level, a.pos0 = k.pos0, a.n_limbs = k.n_limbs;
   a.wide_primes = k.primes_above(32);
-  for (const DevCtx& dc : launch_dcs(c)) launch_linattn(dc, a, (hipStream_t)s);
+  DcList l = launch_dcs(c);
+  for (u32 i = 0; i < l.n; ++i) {
+    l.d[i].N = c->hp.N;  // (a context without a device has none there)
+    if (!linattn_fits(l.d[i], a) || a.n_limbs > 65535) return k.bad("too many results for one call");
+  }
+  if (int e = check_dev(c)) return e;
+  for (const DevCtx& dc : l) launch_linattn(dc, a, (hipStream_t)s);
   stat(ST_LINATTN, (u64)a.n_heads * a.M * a.Nn, polys * 8ull * c->hp.N * k.n_limbs);
   return post_launch();
 }

@@ -536,18 +536,27 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void linattn_shared_kernel
           *(GLOBAL u64*)((GLOBAL char*)uniform(y + (m0 + i) * a.out.row + (j0 + j) * a.out.col + p * a.out.comp) + at) = s[i][j][p].value(red);
 }
 
+// Lanes along x of the launches below.
+template <int NT, int WN, int KW>
+static u64 lanes_rows(const DevCtx& c, const LinattnArgs& a) {
+  return (u64)((c.N + 63) / 64) * a.M * ((a.Nn + NT * WN - 1) / (NT * WN)) * a.n_heads * (64 * WN * KW);
+}
+template <int MT, int NT, int WM, int WN>
+static u64 lanes_shared(const DevCtx& c, const LinattnArgs& a) {
+  return (u64)(c.N / 64) * Tiles(a, MT * WM, NT * WN).all * a.n_heads * (64 * WM * WN);
+}
 template <int NT, int WN, int KW, bool WIDE>
 static void launch_rows(const DevCtx& c, const LinattnArgs& a, hipStream_t s) {
-  const u32 n_blocks = (c.N + 63) / 64, n_tiles = (a.Nn + NT * WN - 1) / (NT * WN);
-  hipLaunchKernelGGL((linattn_kernel<NT, WN, KW, WIDE>), dim3(n_blocks * a.M * n_tiles * a.n_heads, a.n_limbs, c.nrep), dim3(64 * WN * KW), 0, s, c, a, n_blocks, n_tiles);
+  const u32 n_blocks = (c.N + 63) / 64, n_tiles = (a.Nn + NT * WN - 1) / (NT * WN), block = 64 * WN * KW;
+  hipLaunchKernelGGL((linattn_kernel<NT, WN, KW, WIDE>), dim3(lanes_rows<NT, WN, KW>(c, a) / block, a.n_limbs, c.nrep), dim3(block), 0, s, c, a, n_blocks, n_tiles);
 }
 
 template <int MT, int NT, int WM, int WN, int KS, int MIN_WAVES>
 static void launch_shared(const DevCtx& c, const LinattnArgs& a, hipStream_t s) {
   const Tiles tiles(a, MT * WM, NT * WN);
-  const u32 n_blocks = c.N / 64;
+  const u32 n_blocks = c.N / 64, block = 64 * WM * WN;
   if (tiles.all == 0) return;  // (no query sees a key)
-  hipLaunchKernelGGL((linattn_shared_kernel<MT, NT, WM, WN, KS, MIN_WAVES>), dim3(n_blocks * tiles.all * a.n_heads, a.n_limbs, c.nrep), dim3(64 * WM * WN), 0, s, c, a,
+  hipLaunchKernelGGL((linattn_shared_kernel<MT, NT, WM, WN, KS, MIN_WAVES>), dim3(lanes_shared<MT, NT, WM, WN>(c, a) / block, a.n_limbs, c.nrep), dim3(block), 0, s, c, a,
                      n_blocks, tiles);
 }
 
@@ -559,15 +568,36 @@ static void launch_shared(const DevCtx& c, const LinattnArgs& a, hipStream_t s) 
 // One row: its operands are read once whatever the form, and waiting for each other costs (48 x 48 state at N = 8192: 0.72 ms, 0.86 shared) unless half the
 // places stay empty (48 x 48 at 1024, three limbs: 31 us, 27 shared).  Two rows or more share (2 x 40 x 4 scores at 8192: 53 us, 91 unshared by tiles of
 // 4 x 8; 64 x 2 state of four tokens 0.55 ms, 1.09).
-void launch_linattn(const DevCtx& c, const LinattnArgs& a, hipStream_t s) {
+enum class Form { GENERAL, JOINT, SMALL_TILES, TILES, ROWS };
+static Form form(const DevCtx& c, const LinattnArgs& a) {
   const bool row = a.M == 1;
   const u64 blocks = (u64)((c.N + 63) / 64) * a.n_heads * a.n_limbs * c.nrep, small = Tiles(a, 2, 2).all, large = Tiles(a, 4, 4).all;
   const bool spare = row ? blocks * ((a.Nn + 15) / 16) < 512 : blocks * small <= 1024 || small * 20 < large * 43;
-  if (!a.wide_primes)                                                 launch_rows<1, 1, 1, false>(c, a, s);
-  else if (blocks * a.M * a.Nn <= 2048 && (u64)a.t1.K + a.t2.K >= 16) launch_rows<1, 1, 4, true>(c, a, s);
-  else if (c.N >= 64 && spare)                                        launch_shared<1, 1, 2, 2, 2, 4>(c, a, s);
-  else if (c.N >= 64 && !row)                                         launch_shared<2, 2, 2, 2, 1, 4>(c, a, s);
-  else                                                                launch_rows<4, 4, 1, true>(c, a, s);
+  if (!a.wide_primes) return Form::GENERAL;
+  if (blocks * a.M * a.Nn <= 2048 && (u64)a.t1.K + a.t2.K >= 16) return Form::JOINT;
+  if (c.N >= 64 && spare) return Form::SMALL_TILES;
+  return c.N >= 64 && !row ? Form::TILES : Form::ROWS;
+}
+bool linattn_fits(const DevCtx& c, const LinattnArgs& a) {
+  if ((unsigned __int128)((c.N + 63) / 64) * a.M * a.Nn * a.n_heads >> 30) return false;  // (counts of tiles stay in 32 bits; more than any form takes)
+  u64 lanes = 0;
+  switch (form(c, a)) {
+    case Form::GENERAL: lanes = lanes_rows<1, 1, 1>(c, a); break;
+    case Form::JOINT: lanes = lanes_rows<1, 1, 4>(c, a); break;
+    case Form::SMALL_TILES: lanes = lanes_shared<1, 1, 2, 2>(c, a); break;
+    case Form::TILES: lanes = lanes_shared<2, 2, 2, 2>(c, a); break;
+    case Form::ROWS: lanes = lanes_rows<4, 4, 1>(c, a); break;
+  }
+  return lanes >> 32 == 0;
+}
+void launch_linattn(const DevCtx& c, const LinattnArgs& a, hipStream_t s) {
+  switch (form(c, a)) {
+    case Form::GENERAL: return launch_rows<1, 1, 1, false>(c, a, s);
+    case Form::JOINT: return launch_rows<1, 1, 4, true>(c, a, s);
+    case Form::SMALL_TILES: return launch_shared<1, 1, 2, 2, 2, 4>(c, a, s);
+    case Form::TILES: return launch_shared<2, 2, 2, 2, 1, 4>(c, a, s);
+    case Form::ROWS: return launch_rows<4, 4, 1, true>(c, a, s);
+  }
 }
 
 }  // namespace acehip

@@ -74,6 +74,7 @@ struct LinattnArgs {
   u32 level, pos0, n_limbs;
   bool wide_primes = false;        // every prime of the call is above 2^32 and up to 2^64 / 9
 };
+bool linattn_fits(const DevCtx& c, const LinattnArgs& a);  // the launch has less than 2^32 lanes along x
 void launch_linattn(const DevCtx& c, const LinattnArgs& a, hipStream_t s);
 
 }  // namespace acehip

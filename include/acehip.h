@@ -388,7 +388,8 @@ int acehip_rope(acehip_ctx* ctx, const acehip_mat* out, const acehip_mat* in, co
 /* Linear attention with a decay for each head.  (x) is the product of two ciphertexts before relinearisation, (a0, a1) (x) (b0, b1) =
  * (a0 b0, a0 b1 + a1 b0, a1 b1): operands have two polynomials, results three.  Head h reads the keys and values of head
  * h' = h / (n_heads / n_kv_heads).  Rows of q, key, v are tokens, columns features.
- * Counts of tokens and features are below 2^31.
+ * Counts of tokens and features are below 2^31.  A call takes just under 2^34 / N results (heads x rows x columns; any shape of them up to
+ * 2^30 / N); more are refused, and go in calls for some of the heads or rows.
  * A chunk of a prompt: scores (relinearise, rescale), out with the state so far, state.  One token (recurrent form): state with n_k = 1
  * (relinearise, rescale), then out with n_q = 1 and no scores.
  *

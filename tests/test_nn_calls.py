@@ -104,3 +104,32 @@ def test_tables_between_results(rt):  # noqa: F811
     assert changed(Messages, cos=BASE, sin=BASE + 80, os=19).call(rt) == EINVAL
     assert changed(Messages, cos=BASE, sin=BASE + FAR, os=30, pos=BASE + 80, ps=30).call(rt) == ENODEV, rt.err()
     assert changed(Messages, cos=BASE, sin=BASE + FAR, os=30, pos=BASE + 80, ps=10).call(rt) == EINVAL
+
+
+# ---- how much one launch takes -----------------------------------------------------------------------------------------------------------
+@pytest.fixture(scope="module")
+def large():
+    """the ring of the networks"""
+    r = A.AceHip(65536, 2, 60, 56, 1, host_only=True)
+    yield r
+    r.close()
+
+
+def attention(cls, heads, rows, cols, n, **new):
+    """a call with heads x rows x cols results, one limb of a ring of n, all operands broadcast"""
+    out, one = Mat(1 << 50, 3 * n * rows * cols, 3 * n * cols, 3 * n, n), Mat(1 << 12, 0, 0, 0, 0)
+    size = {Scores: dict(nq=rows, nk=cols, q=one, k=one), Out: dict(nq=rows, dv=cols, q=one, S=one, p=one, v=one, din=None, decay=None),
+            State: dict(dk=rows, dv=cols, S=one, k=one, v=one, keep=None, decay=None)}[cls]
+    return changed(cls, out=out, heads=heads, kv=1, level=1, n=1, **size, **new)
+
+
+@pytest.mark.parametrize("cls", [Scores, Out, State], ids=lambda c: c.__name__)
+@pytest.mark.parametrize("heads,rows,cols", [(4, 64, 64), (1, 128, 128), (8, 128, 128), (16, 64, 252), (3, 61, 67), (2048, 1, 16), (1, 1, 1 << 17), (1, 1, (1 << 18) - 16), ((1 << 14) - 1, 1, 1), (1, (1 << 15) - 2, 1), (1, 2, 1 << 14)])
+def test_results_of_one_call(large, cls, heads, rows, cols):
+    assert attention(cls, heads, rows, cols, large.N).call(large) == ENODEV, large.err()
+
+
+@pytest.mark.parametrize("cls", [Scores, Out, State], ids=lambda c: c.__name__)
+@pytest.mark.parametrize("heads,rows,cols", [(8, 256, 256), (1, 1 << 15, 1 << 15), (1, 1, 1 << 19), (1 << 31, 1, 1), (1, 1 << 16, 1 << 16)])
+def test_too_many_results(large, cls, heads, rows, cols):
+    assert attention(cls, heads, rows, cols, large.N).call(large) == EINVAL and "too many" in large.err()
