@@ -243,7 +243,10 @@ int acehip_linear_i8(acehip_ctx* c, const acehip_mat* out, const acehip_mat* in,
   // (weights inside the arena differ from replica to replica: they are read as they lie)
   const bool shared = c->dc.rep_span == 0 || (u64)(uintptr_t)d_w - c->dc.rep_lo >= c->dc.rep_span;
   const DcList l = launch_dcs(c);
-  launch_linear(c->dc, l.d, l.n, a, shared ? c->ws : nullptr, c->ws_words * sizeof(u64), (hipStream_t)s);
+  // one copy for all replicas of the call, in the workspace of the first: what is not selected stays as it is
+  const bool moved = (u64)(uintptr_t)c->ws - c->dc.rep_lo < c->dc.rep_span;
+  u64* const ws = c->ws + (moved ? l.d[0].rep0 * (c->dc.rep_stride / sizeof(u64)) : 0);
+  launch_linear(c->dc, l.d, l.n, a, shared ? ws : nullptr, c->ws_words * sizeof(u64), (hipStream_t)s);
   const u64 limb = 8ull * c->hp.N * n_limbs * rows;
   stat(ST_LINEAR, (u64)rows * n_out, limb * ((u64)n_comp * n_in + (u64)n_comp * n_out + (d_tok ? 1 : 0)) + (u64)n_in * n_out);
   return post_launch();

@@ -1,4 +1,6 @@
 """GPU tests (-m gpu) of the operators on ciphertexts at the calls that tests/test_gpu_nn.py leaves out: packed weights of every kind, large rings."""
+import ctypes as C
+
 import numpy as np
 import pytest
 from test_gpu_nn import LargeAttn, Sampled, contexts, dev, linear_case, pair  # noqa: F401  (a fixture)
@@ -94,3 +96,92 @@ def test_many_results_in_the_largest_ring(large):
         assert np.array_equal(got.reshape(3, N)[:, at], want.astype(np.uint64)), (h, t, s)
     for b in (dx, dk, dy):
         b.free()
+
+
+# ---- packed weights: where they lie, and what reads them -----------------------------------------------------------------------------------
+class Arena:
+    """a context whose polynomials and workspace lie in memory that the test sees, `n_rep` times; a linear layer of ROWS rows that share their inputs,
+    large enough a launch for its weights to be packed"""
+
+    N, LEVEL, ROWS, COMPS = 64, 3, 48, 2
+
+    def __init__(self, n_rep, n_in, n_out, ld, seed=1):
+        self.rt = rt = A.AceHip(self.N, 7, 60, 51, 3)
+        self.poly, self.n_in, self.n_out, self.ld, self.n_rep = self.LEVEL * self.N, n_in, n_out, ld, n_rep
+        self.rng = np.random.default_rng(seed)
+        ws = int(rt.lib.acehip_workspace_words(rt.h))
+        sizes = dict(x=n_in * self.COMPS * self.poly, y=self.ROWS * n_out * self.COMPS * self.poly, w=(n_out * ld + 64) // 8, ws=ws, scratch=64 * self.N)
+        self.at, self.total = {}, 0
+        for k, n in sizes.items():
+            self.at[k] = (self.total, n)
+            self.total += n + n % 2
+        self.base = rt.buf(self.total * n_rep)
+        cfg = A.binding.ArenaCfg(self.base.ptr, self.total * 8, self.total * 8, n_rep, self.ptr("ws"), self.ptr("scratch"), 64)
+        rt.check(rt.lib.acehip_ctx_set_arena(rt.h, C.byref(cfg)))
+        self.host = np.zeros((n_rep, self.total), np.uint64)
+        self.q = np.array(rt.primes[: self.LEVEL], dtype=object)[:, None]
+
+    def ptr(self, k):
+        return self.base.ptr + 8 * self.at[k][0]
+
+    def part(self, words, k):
+        return words[:, self.at[k][0]: sum(self.at[k])]
+
+    def fill(self):
+        """new inputs; results and workspace cleared"""
+        x = np.stack([self.rng.integers(0, int(p), size=(self.n_rep, self.n_in, self.COMPS, self.N), dtype=np.uint64) for p in self.q[:, 0]], axis=-2)
+        self.host[:] = 0
+        self.part(self.host, "x")[:] = x.reshape(self.n_rep, -1)
+        self.base.upload(self.host)
+        return x
+
+    def weights(self, *lead):
+        return self.rng.integers(-128, 128, size=(*lead, self.n_out, self.ld)).astype(np.int8)
+
+    def call(self, d_w, stream=None):
+        self.rt.linear_i8(self.rt.mat(self.ptr("y"), 0, self.n_out * self.COMPS * self.poly, self.COMPS * self.poly, self.poly), self.rt.mat(self.ptr("x"), 0, 0, self.COMPS * self.poly, self.poly),
+                          d_w, self.ld, self.ROWS, self.n_in, self.n_out, self.COMPS, self.LEVEL, stream=stream)
+
+    def memory(self):
+        self.rt.sync()
+        return self.base.download((self.n_rep, self.total))
+
+    def want(self, w, x):
+        """of one row and replica: [output][polynomial][limb][N]"""
+        return (np.tensordot(w[:, : self.n_in].astype(object), x.astype(object), (1, 0)) % self.q).astype(np.uint64)
+
+    def results(self, words):
+        return self.part(words, "y").reshape(self.n_rep, self.ROWS, self.n_out, self.COMPS, self.LEVEL, self.N)
+
+    def close(self):
+        self.base.free()
+        self.rt.close()
+
+
+def test_packed_weights_under_a_selection():
+    """replicas 1 and 2 of three: they share packed weights, and nothing of replica 0 changes, its workspace neither; weights in the arena are each
+    replica's own and are read as they lie"""
+    a = Arena(3, 20, 40, 23)
+    x, w, own = a.fill(), a.weights(), a.weights(3)
+    dw = dev(a.rt, w)
+    a.rt.check(a.rt.lib.acehip_ctx_select(a.rt.h, 1, 2))
+    a.call(dw.ptr)
+    got = a.memory()
+    assert a.part(got, "ws").any()
+    assert np.array_equal(got[0], a.host[0])
+    for r in (1, 2):
+        y = a.results(got)[r]
+        assert np.array_equal(y, np.broadcast_to(a.want(w, x[r]), y.shape))
+    x = a.fill()
+    for r in range(3):
+        a.part(a.host, "w")[r].view(np.int8)[: own[r].size] = own[r].ravel()
+    a.base.upload(a.host)
+    a.call(a.ptr("w"))
+    got = a.memory()
+    assert not a.part(got, "ws").any()
+    assert np.array_equal(got[0], a.host[0])
+    for r in (1, 2):
+        y = a.results(got)[r]
+        assert np.array_equal(y, np.broadcast_to(a.want(own[r], x[r]), y.shape))
+    dw.free()
+    a.close()
