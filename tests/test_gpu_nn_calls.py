@@ -1,9 +1,10 @@
 """GPU tests (-m gpu) of the operators on ciphertexts at the calls that tests/test_gpu_nn.py leaves out: packed weights of every kind, large rings."""
 import ctypes as C
+import itertools
 
 import numpy as np
 import pytest
-from test_gpu_nn import LargeAttn, Sampled, contexts, dev, linear_case, pair  # noqa: F401  (a fixture)
+from test_gpu_nn import LargeAttn, Sampled, contexts, dev, hip, linear_case, ok, pair  # noqa: F401  (a fixture)
 
 import ace_compiler_amd as A
 
@@ -158,6 +159,20 @@ class Arena:
         self.rt.close()
 
 
+@pytest.mark.parametrize("n_in,n_out,ld,w_off", [(70, 40, 70, 0), (70, 40, 71, 1), (70, 70, 80, 16), (70, 33, 77, 3), (64, 129, 64, 5), (1, 40, 1, 1), (65, 200, 67, 2)])
+def test_packed_weights_of_any_alignment(n_in, n_out, ld, w_off):
+    a = Arena(1, n_in, n_out, ld)
+    x, w = a.fill(), a.weights()
+    dw = dev(a.rt, np.concatenate([np.zeros(w_off, np.int8), w.ravel()[: (n_out - 1) * ld + n_in]]))
+    a.call(dw.ptr + w_off)
+    got = a.memory()
+    assert a.part(got, "ws").any()  # packed
+    y = a.results(got)[0]
+    assert np.array_equal(y, np.broadcast_to(a.want(w, x[0]), y.shape))
+    dw.free()
+    a.close()
+
+
 def test_packed_weights_under_a_selection():
     """replicas 1 and 2 of three: they share packed weights, and nothing of replica 0 changes, its workspace neither; weights in the arena are each
     replica's own and are read as they lie"""
@@ -184,4 +199,61 @@ def test_packed_weights_under_a_selection():
         y = a.results(got)[r]
         assert np.array_equal(y, np.broadcast_to(a.want(own[r], x[r]), y.shape))
     dw.free()
+    a.close()
+
+
+def test_packed_weights_of_simulated_ranks():
+    a = Arena(2, 20, 40, 20)
+    a.rt.check(a.rt.lib.acehip_ctx_shard_sim(a.rt.h, 2))
+    x, w = a.fill(), a.weights()
+    a.part(a.host, "x")[1] = a.part(a.host, "x")[0]
+    a.base.upload(a.host)
+    dw = dev(a.rt, w)
+    a.call(dw.ptr)
+    got = a.memory()
+    assert a.part(got, "ws").any()
+    want = a.want(w, x[0])
+    for r, l in itertools.product(range(2), range(a.LEVEL)):
+        y = a.results(got)[r, ..., l, :]
+        assert np.array_equal(y, np.broadcast_to(want[..., l, :], y.shape)) if l % 2 == r else not y.any()
+    dw.free()
+    a.close()
+
+
+def test_packed_weights_in_a_graph():
+    """two layers that pack into the same workspace in one graph, replayed on new inputs and weights with eager calls in between"""
+    a = Arena(1, 70, 40, 70)
+    lib = hip()
+    w = a.weights(2)
+    dw = [dev(a.rt, v) for v in w]
+    x = a.fill()
+    st, graph, run = C.c_void_p(), C.c_void_p(), C.c_void_p()
+    ok(lib.hipStreamCreateWithFlags(C.byref(st), 1))
+    keep = a.rt.buf(a.at["y"][1])  # the first layer's results
+    ok(lib.hipStreamBeginCapture(st, 1))  # thread-local
+    y = a.rt.mat(keep.ptr, 0, a.n_out * a.COMPS * a.poly, a.COMPS * a.poly, a.poly)
+    a.rt.linear_i8(y, a.rt.mat(a.ptr("x"), 0, 0, a.COMPS * a.poly, a.poly), dw[0].ptr, a.ld, a.ROWS, a.n_in, a.n_out, a.COMPS, a.LEVEL, stream=st)
+    a.call(dw[1].ptr, stream=st)
+    ok(lib.hipStreamEndCapture(st, C.byref(graph)))
+    ok(lib.hipGraphInstantiate(C.byref(run), graph, None, None, 0))
+    for _ in range(4):
+        x, w = a.fill(), a.weights(2)
+        for d, v in zip(dw, w):
+            d.upload(v.ravel())
+        a.rt.sync()
+        ok(lib.hipGraphLaunch(run, st))
+        ok(lib.hipStreamSynchronize(st))
+        got = a.memory()
+        assert a.part(got, "ws").any()
+        for words, v in ((keep.download((1, -1)), w[0]), (a.part(got, "y"), w[1])):
+            y = words.reshape(a.ROWS, a.n_out, a.COMPS, a.LEVEL, a.N)
+            assert np.array_equal(y, np.broadcast_to(a.want(v, x[0]), y.shape))
+        a.call(dw[0].ptr)
+        y = a.results(a.memory())[0]
+        assert np.array_equal(y, np.broadcast_to(a.want(w[0], x[0]), y.shape))
+    ok(lib.hipGraphExecDestroy(run))
+    ok(lib.hipGraphDestroy(graph))
+    ok(lib.hipStreamDestroy(st))
+    for d in (*dw, keep):
+        d.free()
     a.close()
