@@ -398,8 +398,9 @@ int acehip_rope(acehip_ctx* ctx, const acehip_mat* out, const acehip_mat* in, co
 int acehip_linattn_scores(acehip_ctx* ctx, const acehip_mat* p3, const acehip_mat* q, const acehip_mat* key, uint32_t n_heads, uint32_t n_kv_heads,
                           uint32_t n_q, uint32_t n_k, uint32_t dim, int causal, uint32_t level, uint32_t pos0, uint32_t n_limbs, acehip_stream stream);
 /* o3[h][t][b] = in[h][t] * sum_{a < dim_k} q[t][h][a] (x) state[h][a][b] + sum_s decay[h][t + n_k - n_q - s] * p[h][t][s] (x) v[s][h'][b]
- * q and state, p and v may be NULL (both of a pair): that sum is empty.  causal: s <= t + n_k - n_q, the other p are not read; otherwise all
- * s < n_k, and d_decay is NULL.  d_in: [n_heads][n_q], d_decay: [n_heads][n_k] by distance; NULL: 1. */
+ * q and state, p and v may be NULL (both of a pair): that sum is empty.  causal: s <= t + n_k - n_q, the other p have no influence, whatever
+ * they hold (some are read all the same: they lie in memory of the caller); otherwise all s < n_k, and d_decay is NULL.  d_in: [n_heads][n_q],
+ * d_decay: [n_heads][n_k] by distance; NULL: 1. */
 int acehip_linattn_out(acehip_ctx* ctx, const acehip_mat* o3, const acehip_mat* q, const acehip_mat* state, const acehip_mat* p, const acehip_mat* v,
                        uint32_t n_heads, uint32_t n_kv_heads, uint32_t n_q, uint32_t n_k, uint32_t dim_k, uint32_t dim_v, const int64_t* d_in,
                        const int64_t* d_decay, int causal, uint32_t level, uint32_t pos0, uint32_t n_limbs, acehip_stream stream);

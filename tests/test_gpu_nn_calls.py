@@ -4,7 +4,7 @@ import itertools
 
 import numpy as np
 import pytest
-from test_gpu_nn import LargeAttn, Sampled, contexts, dev, hip, linear_case, ok, pair  # noqa: F401  (a fixture)
+from test_gpu_nn import Attn, LargeAttn, Sampled, _open, contexts, dev, hip, linear_case, ok, pair  # noqa: F401  (a fixture)
 
 import ace_compiler_amd as A
 
@@ -97,6 +97,24 @@ def test_many_results_in_the_largest_ring(large):
         assert np.array_equal(got.reshape(3, N)[:, at], want.astype(np.uint64)), (h, t, s)
     for b in (dx, dk, dy):
         b.free()
+
+
+# ---- what the mask leaves out --------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("name,args,cls", [("n64", None, Attn), ("n16", None, Attn), ("n32", None, Attn), ("n16384", (16384, 2, 60, 50, 1), LargeAttn)])
+@pytest.mark.parametrize("sizes", [(2, 1, 5, 5, 2, 3), (1, 1, 7, 4, 13, 5), (1, 1, 3, 70, 2, 2)], ids=str)
+def test_unseen_scores_hold_anything(contexts, name, args, cls, sizes):  # noqa: F811
+    """p[h][t][s] of keys that query t does not see: no residues, all bits set"""
+    rt = contexts(name) if args is None else _open.setdefault(name, A.AceHip(*args))
+    a = cls(rt, 2, [0, 1], *sizes)
+    H, kv, nq, nk, dk, dv = sizes
+    for ix, _, words in a.p.spots(a.p.host):
+        if ix[2] > ix[1] + nk - nq:
+            words[:] = ~np.uint64(0)
+    a.p.buf.upload(a.p.host)
+    a.out()
+    a.out(factor=False)
+    a.out(state=False)
+    a.free()
 
 
 # ---- packed weights: where they lie, and what reads them -----------------------------------------------------------------------------------
