@@ -207,9 +207,10 @@ def prepare(case, seed):
         if c.get("chunk"):
             st["P"] = uniform(H, n, n, 2)
         st["y"] = zeros(H, *{"scores": (n, n), "out": (n, c.get("dv")), "state": (c["dk"], c.get("dv"))}[c["op"]], 3)
-    if own:  # the handle that a program keeps: the context of its parameter set, and the stream that it works on
+    if own:  # the handle that a program keeps: the context of its parameter set, and the stream that it works on -- one for a context, whose
+        # calls may share its workspace and follow each other
         st["rt"] = _context(1024 if c["op"] == "angles" else N)
-        st["stream"] = torch.cuda.Stream()
+        st["stream"] = _stream(1024 if c["op"] == "angles" else N)
         torch.cuda.synchronize()
     return st
 
@@ -221,6 +222,11 @@ def _context(N):
     rt = A.AceHip(N, *SETS[N])
     assert rt.primes[: rt.L] == _primes(N)
     return rt
+
+
+@functools.lru_cache(None)
+def _stream(N):
+    return torch.cuda.Stream()
 
 
 # ---- one pass -------------------------------------------------------------------------------------------------------------------------
