@@ -36,3 +36,15 @@ def test_packed_weights_are_read_inside_their_array(linear_parts, n_in, ld, rest
     rc, got = linear_parts(64, 30, n_in, 2 * part + rest, ld, workspace)
     assert rc == 0 and got["bad"] == 0, got
     assert got["packs"] == 2 + (rest > 32) and got["products"] == 2 + (rest > 0), got
+
+
+@pytest.mark.parametrize("kind", ["asan", "tsan"])
+def test_argument_checks_under_sanitizer(kind):
+    """tests/c/san_nn.cpp: random calls of every entry point, from one thread and from four"""
+    if not os.path.exists(HIPCC):
+        pytest.skip("hipcc not available")
+    subprocess.check_call(["make", "-s", "-C", os.path.join(ROOT, "oracle"), kind + "_nn"])
+    env = dict(os.environ, ASAN_OPTIONS="detect_leaks=1:abort_on_error=0", UBSAN_OPTIONS="print_stacktrace=1:halt_on_error=1", TSAN_OPTIONS="halt_on_error=1")
+    r = subprocess.run([os.path.join(ROOT, "oracle", "_san", "san_nn_" + kind)], capture_output=True, text=True, timeout=600, env=env)
+    assert r.returncode == 0 and "san_nn: OK" in r.stdout, (r.stdout[-2000:], r.stderr[-4000:])
+    assert "ERROR: " not in r.stderr and "WARNING: ThreadSanitizer" not in r.stderr, r.stderr[-4000:]
