@@ -84,8 +84,8 @@ __device__ __forceinline__ u64 mul_near(u64 a, u64 w, u64 wp, u64 nq) {
 
 // Column blocks of a launch: 16 WN columns of one polynomial of one row.
 struct Columns {
-  u32 first, step, n;  // of a workgroup: column blocks first, first + step ..
-  u32 log_blocks;      // column blocks of a polynomial
+  u32 first, n;    // of a workgroup
+  u32 log_blocks;  // column blocks of a polynomial
 };
 
 template <int NP, int MT, int WJ, int WN, bool PACKED, bool ODD>
@@ -99,7 +99,7 @@ __device__ __forceinline__ void linear_tiles(const DevCtx& c, const LinearArgs& 
   const u64 q = P.q, mh = P.prec128_hi;
   // where a column block starts in a matrix (uniform)
   auto block = [&](u32 i, const CtMat& m, u64* base, u32& row, u64& off) {
-    const u32 cb = cols.first + i * cols.step, rc = cb >> cols.log_blocks;
+    const u32 cb = cols.first + i, rc = cb >> cols.log_blocks;
     row = __builtin_amdgcn_readfirstlane(rc / a.n_comp);
     const u32 comp = rc - row * a.n_comp;
     off = (u64)pos * c.N + (cb & ((1u << cols.log_blocks) - 1)) * (16 * WN);
@@ -346,7 +346,7 @@ __device__ __forceinline__ void linear_tiles(const DevCtx& c, const LinearArgs& 
   }
 }
 
-// A workgroup takes `tiles` column blocks one after the other; the rest of them go by launch_mfma's order.
+// A workgroup takes `tiles` column blocks that follow each other (the last workgroup what is left).
 template <int MT, int WJ, int WN, bool PACKED, bool ODD>
 __global__ __launch_bounds__(64 * WJ * WN, 2) void linear_i8_mfma_kernel(DevCtx c, LinearArgs a, u32 j_blocks, u32 log_blocks, u32 tiles) {
   __shared__ v4i_t frag[2 * WN * 8 * 64];
@@ -368,7 +368,7 @@ __global__ __launch_bounds__(64 * WJ * WN, 2) void linear_i8_mfma_kernel(DevCtx 
   if (!owns(c, gi)) return;
   const DevPrime P = c.primes[gi];
   const u32 all = (a.rows * a.n_comp) << log_blocks;
-  const Columns cols{g * tiles, 1, min(tiles, all - g * tiles), log_blocks};
+  const Columns cols{g * tiles, min(tiles, all - g * tiles), log_blocks};
   const u32 j0 = jb * (16 * MT * WJ);
   if (P.q <= kBytes7) linear_tiles<7, MT, WJ, WN, PACKED, ODD>(c, a, frag, factor, P, rep, pos, cols, j0);
   else                linear_tiles<8, MT, WJ, WN, PACKED, ODD>(c, a, frag, factor, P, rep, pos, cols, j0);
