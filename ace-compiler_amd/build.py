@@ -64,7 +64,7 @@ FPR_TAG = b"ACEHIP_SRC_FPR="
 def hip_flags():
     """the flags every HIP object is compiled with.  -fgpu-default-stream=per-thread: the NULL stream of every entry point is the
     calling thread's own stream, so host threads that each own a context (one image stream each) run concurrently on the GPU.
-    -packed-fp32-ops: no packed single-precision instructions, some forms of which have given wrong results now and then.
+    -packed-fp32-ops: no packed single-precision instructions.
     ACEHIP_EXTRA_HIPCC_FLAGS: experiments only; part of the fingerprint, so a process that does not carry the same value refuses
     (rebuilds) a library built with it."""
     return ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-x", "hip", "-fgpu-default-stream=per-thread", "-Wall",

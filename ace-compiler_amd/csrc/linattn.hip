@@ -33,12 +33,6 @@ struct Reduce {
     near_q = __builtin_fmaf((float)(u32)(ml >> 32), 0x1p-32f, (float)mh) * (0x1p-32f * 0.999999f);
   }
 };
-// a * w mod q up to multiples of q: below 5q for any a, with a companion wp of w that is at most two units of 2^-64 too small (the quotient leaves
-// out the low product and two carries)
-__device__ __forceinline__ u64 mul_near(u64 a, u64 w, u64 wp, u64 nq) {
-  const u64 h = (u64)(u32)(a >> 32) * (u32)(wp >> 32) + __umulhi((u32)(a >> 32), (u32)wp) + __umulhi((u32)a, (u32)(wp >> 32));
-  return a * w + h * nq;
-}
 struct Acc {
   u64 ll, mm, hh;
   __device__ __forceinline__ void mac(const Half& x, const Half& y) {
@@ -81,12 +75,8 @@ struct Acc {
   }
 };
 
-#define GLOBAL __attribute__((address_space(1)))
-// a pointer that is the same for the wave, on the scalar unit (lanes add their coefficient as a 32-bit offset)
-__device__ __forceinline__ const GLOBAL char* uniform(const u64* p) {
-  const u64 v = (u64)p;
-  return (const GLOBAL char*)(((u64)(u32)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) | (u32)__builtin_amdgcn_readfirstlane((int)v));
-}
+// a pointer that is the same for the wave (lanes add their coefficient as a 32-bit offset)
+__device__ __forceinline__ const GLOBAL char* uniform(const u64* p) { return (const GLOBAL char*)uniform64((u64)p); }
 
 // One row of results.  A wave: 64 coefficients, NT results (3 sums of 3 words each) over every KW-th term; a workgroup: WN waves along the columns, KW along
 // the terms, whose sums are joined through LDS.  Per term of the sums a lane reads 2 (1 + NT) residues and makes 12 NT multiply-adds.
@@ -277,11 +267,6 @@ __global__ __launch_bounds__(64 * WN * KW, 2) void linattn_kernel(DevCtx c, Lina
 // Sums of int8 products on the matrix cores, as in linear.hip, cost as many instructions: tiles of 16 x 16 leave a byte 16 uses for its transposition,
 // and the reductions at the end weigh more at sums this short; that form took 1.63 ms.
 // Tiles of 2 x 2 results in 2 x 2 waves: 2 x 4 results (half the waves) 1.56 ms, 2 x 4 waves 1.52, two terms a stage 1.16.
-__device__ __forceinline__ void lds_barrier() {  // LDS writes are visible, requests to memory stay in flight
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
 // The tiles of a launch, row by row, without those of causal scores that no query sees (workgroups that end at once come in a pattern that leaves some
 // of the shader engines, which take workgroups in turn, without work: 32 x 32 scores 1.01 ms in place of 0.90).  Row tm of tiles has
 // tm + lead of them, between 0 and n: rows r0 .. r0 + grow - 1 have c0, c0 + 1, ..; the rows behind all n.

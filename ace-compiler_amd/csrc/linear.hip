@@ -22,19 +22,14 @@ namespace acehip {
 // ------------------------------------------------------------------------------------------------
 typedef int v4i_t __attribute__((ext_vector_type(4)));
 typedef int v4i_any_t __attribute__((ext_vector_type(4), aligned(1)));
-// global address space spelled out: FLAT loads would count as LDS accesses too, and every wait for LDS would wait for them
-#define GLOBAL __attribute__((address_space(1)))
 template <class T>
 __device__ __forceinline__ GLOBAL T* global(T* p) { return (GLOBAL T*)(uintptr_t)p; }
 constexpr u64 kBytes7 = 0x7f7f7f7f7f7f7full;  // the largest residue of seven signed bytes
 
 __device__ __forceinline__ u32 perm(u32 hi, u32 lo, u32 sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
-// a pointer that is the same for the wave, kept on the scalar unit
+// a pointer that is the same for the wave
 template <class T>
-__device__ __forceinline__ T* uniform(T* p) {
-  const u64 v = (u64)p;
-  return (T*)(((u64)(u32)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) | (u32)__builtin_amdgcn_readfirstlane((int)v));
-}
+__device__ __forceinline__ T* uniform(T* p) { return (T*)uniform64((u64)p); }
 // bytes of four dwords transposed: o[b] = byte b of l[0..3]
 __device__ __forceinline__ void transpose4(const u32 (&l)[4], u32 (&o)[4]) {
   const u32 a01 = perm(l[1], l[0], 0x05010400u), a23 = perm(l[3], l[2], 0x05010400u);
@@ -43,12 +38,6 @@ __device__ __forceinline__ void transpose4(const u32 (&l)[4], u32 (&o)[4]) {
   o[1] = perm(a23, a01, 0x07060302u);
   o[2] = perm(b23, b01, 0x05040100u);
   o[3] = perm(b23, b01, 0x07060302u);
-}
-// LDS writes of the workgroup are visible, loads from memory stay in flight
-__device__ __forceinline__ void lds_barrier() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 // The first of 16 bytes that hold the weights from byte `at` of the array on, as far as they are there; of an array of 16 bytes at least.
@@ -73,13 +62,6 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const int8_t* w, u64 l
     if (n_in - k < 16) v &= ((unsigned __int128)1 << (8 * (n_in - k))) - 1;
   }
   out[(u64)f * 64 + lane] = __builtin_bit_cast(v4i_t, v);
-}
-
-// a * w mod q up to multiples of q for a < 2^63, with nq = -q and a companion wp of w that is at most two units of 2^-64 too small: below 4q
-// (the quotient leaves out the low product and two carries: at most 3 too small, and a w / q - a wp / 2^64 < 1)
-__device__ __forceinline__ u64 mul_near(u64 a, u64 w, u64 wp, u64 nq) {
-  const u64 h = (u64)(u32)(a >> 32) * (u32)(wp >> 32) + __umulhi((u32)(a >> 32), (u32)wp) + __umulhi((u32)a, (u32)(wp >> 32));
-  return a * w + h * nq;
 }
 
 // Column blocks of a launch: 16 WN columns of one polynomial of one row.

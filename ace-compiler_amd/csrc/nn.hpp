@@ -19,6 +19,25 @@ __device__ __forceinline__ u64 signed_mod(int64_t w, u64 q, u64 mh) {
   return w < 0 && r != 0 ? q - r : r;
 }
 
+// global address space spelled out: FLAT loads would count as LDS accesses too, and every wait for LDS would wait for them
+#define GLOBAL __attribute__((address_space(1)))
+// a word that is the same for the wave, kept on the scalar unit
+__device__ __forceinline__ u64 uniform64(u64 v) {
+  return ((u64)(u32)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) | (u32)__builtin_amdgcn_readfirstlane((int)v);
+}
+// LDS writes of the workgroup are visible, requests to memory stay in flight
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+// a * w mod q up to multiples of q, with nq = -q and a companion wp of w that is at most two units of 2^-64 too small: below 5q, below 4q for a < 2^63
+// (the quotient leaves out the low product and two carries, less than 3; a w / q - a wp / 2^64 is below 2, for a < 2^63 below 1)
+__device__ __forceinline__ u64 mul_near(u64 a, u64 w, u64 wp, u64 nq) {
+  const u64 h = (u64)(u32)(a >> 32) * (u32)(wp >> 32) + __umulhi((u32)(a >> 32), (u32)wp) + __umulhi((u32)a, (u32)(wp >> 32));
+  return a * w + h * nq;
+}
+
 // y[r][j] = tok[r] * mul[j] * sum_i w[j][i] x[r][i], every polynomial of the ciphertexts (linear.hip)
 struct LinearArgs {
   CtMat out, in;
