@@ -262,7 +262,7 @@ __global__ __launch_bounds__(64 * WN * KW, 2) void linattn_kernel(DevCtx c, Lina
 // Bound by the integer instructions, at about four cycles each: 100 for a wave's term of 4 x 64 results without factors (48 multiply-adds, 10 to add halves and
 // read LDS, 14 staging, up to 36 of carries at primes of 60 bits, the rest start and end of a sum of 32 terms), 60 in place of 14 where the staged
 // residues have factors.  32 x 32 causal scores of 32 features, four heads of two, three limbs at N = 4096: 0.90 ms, 10^10 multiply-adds (38 % of the
-// rate they reach alone), 1.8 GB.  A chunk of 16 with a state of 24 x 32, two heads, three limbs at 8192: 1.01 ms, the units for them busy for 85 % of it.
+// rate they reach alone), 1.8 GB.  A chunk of 16 with a state of 24 x 32, two heads, three limbs at 8192: 1.01 ms, the vector units busy for 87 % of it.
 // One token into 32 x 32 states, four heads and limbs at 8192: 1.27 ms for 5.5 GB (4.3 TB/s), bound by memory.
 // Sums of int8 products on the matrix cores, as in linear.hip, cost as many instructions: tiles of 16 x 16 leave a byte 16 uses for its transposition,
 // and the reductions at the end weigh more at sums this short; that form took 1.63 ms.
@@ -545,11 +545,11 @@ static void launch_shared(const DevCtx& c, const LinattnArgs& a, hipStream_t s) 
                      n_blocks, tiles);
 }
 
-// Where a workgroup for each result leaves every workgroup a place (eight on each of 256 CUs), the sums are cut over its waves: 4 x 4 scores of 64 features
-// at N = 1024 8.3 us, 21 by the next form; a 64 x 64 state read by one token 15 and 25; with more of them it loses (16 x 16 states, 16 tokens: 24 us, 20).
-// Tiles of 2 x 2 results, two terms a stage, where their workgroups have a place at once (four on each CU; 9 x 9 scores of 51 features at 2048: 25 us, 38 by
-// 4 x 4; with 1280 workgroups, 8 x 8 scores of 24 features at 4096, 27 and 24), or where 4 x 4 leave more idle than they save: one takes as long as 2.15
-// of 2 x 2 (2 x 2 scores of 40 features, eight heads, three limbs at 8192: 100 us, 124 by 4 x 4; 6 x 6 states, 20 tokens: 359 and 336).
+// Up to 2048 workgroups of a result each (1792 have a place at once, seven on each of 256 CUs), the sums are cut over a workgroup's waves: 4 x 4 scores of 64
+// features at N = 1024 8.3 us, 21 by the next form; a 64 x 64 state read by one token 15 and 25; with more of them it loses (16 x 16 states, 16 tokens: 24
+// us, 20).  Tiles of 2 x 2 results, two terms a stage, up to 1024 workgroups of them (9 x 9 scores of 51 features at 2048: 25 us, 38 by 4 x 4; with 1280
+// workgroups, 8 x 8 scores of 24 features at 4096, 27 and 24), or where 4 x 4 leave more idle than they save: one takes as long as 2.15 of 2 x 2 (2 x 2
+// scores of 40 features, eight heads, three limbs at 8192: 100 us, 124 by 4 x 4; 6 x 6 states, 20 tokens: 359 and 336).
 // One row: its operands are read once whatever the form, and waiting for each other costs (48 x 48 state at N = 8192: 0.72 ms, 0.86 shared) unless half the
 // places stay empty (48 x 48 at 1024, three limbs: 31 us, 27 shared).  Two rows or more share (2 x 40 x 4 scores at 8192: 53 us, 91 unshared by tiles of
 // 4 x 8; 64 x 2 state of four tokens 0.55 ms, 1.09).

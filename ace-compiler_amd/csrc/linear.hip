@@ -15,10 +15,10 @@ namespace acehip {
 // inputs: the residues are read once by the workgroup, their bytes transposed in registers (four inputs of a column by v_perm_b32) and left in LDS
 // as the B fragments of v_mfma_i32_16x16x64_i8 (1 KiB each, read without bank conflicts); the weights are the A fragments, packed by a kernel of
 // their own (or, up to 32 outputs, as their rows lie in memory).  Residues are requested three steps ahead and staged one ahead, weights one.
-// Bound: up to 128 outputs by memory (800 -> 32, N = 16384, two rows, three limbs: 0.28 ms, 4.7 TB/s; 333 -> 77, N = 4096, three rows: 59 us, 4.1 TB/s);
-// above by the matrix cores and the power that they draw (768 -> 2304 at N = 16384: 1.66 ms, 2.78 * 10^15 int8 operations, 1.67 POP/s; the product
-// with its LDS reads and stores alone takes 0.92 ms, staging 0.15, the loads 0.4 and the reduction 0.2: the parts add up since the clock falls to
-// 1.96 GHz; a library's int8 product of 8192^3 reaches 2.08 POP/s on this card).
+// Bound: up to 128 outputs by memory (800 -> 32, N = 16384, two rows, three limbs: 0.28 ms, 4.7 TB/s; 333 -> 77, N = 4096, three rows: 62 us, 3.9 TB/s, of
+// which the packing takes 5); above by parts that follow each other (768 -> 2304 at N = 16384: 1.67 ms, 2.78 * 10^12 int8 operations, 1.67 POP/s, matrix
+// cores busy for 43 % of it at 1.94 GHz: the product with its LDS reads alone takes 1.02 ms, staging adds 0.12, the loads 0.32 and the reduction 0.19;
+// a library's int8 product of 8192^3 reaches 2.07 POP/s on this card).
 // ------------------------------------------------------------------------------------------------
 typedef int v4i_t __attribute__((ext_vector_type(4)));
 typedef int v4i_any_t __attribute__((ext_vector_type(4), aligned(1)));

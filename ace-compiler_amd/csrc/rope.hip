@@ -4,7 +4,7 @@
 namespace acehip {
 
 // The angle is one rounded product of doubles; cos and sin of that double (positions far out lose nothing more).  Two positions a lane, whose
-// latencies overlap.  Bound by its stores and its launch: 32768 positions of 64 pairs, 34 MB, in 7.6 us (4.5 TB/s); replayed in a graph 9.7 us, 10.4 with
+// latencies overlap.  Bound by its stores and its launch: 32768 positions of 64 pairs, 34 MB, in 8.5 us (4.0 TB/s); replayed in a graph 9.7 us, 10.4 with
 // one position a lane, 8.3 without the functions.
 __global__ __launch_bounds__(256) void rope_messages_kernel(double* cos_out, double* sin_out, u64 out_stride, const double* pos, u64 pos_stride, u32 n_pos,
                                                             RopeAngles a) {
@@ -29,7 +29,7 @@ void launch_rope_messages(double* cos_out, double* sin_out, u64 out_stride, cons
 
 // A lane: one coefficient of a pair, whose table it reads once for up to `per` polynomials (heads and components); `parts` workgroups share a
 // pair's polynomials.  Two products a result with 128-bit sums, reduced once: bound by memory, each word read and written once (16 heads of 64 at
-// N = 16384, four limbs: 2.2 GB in 0.436 ms, 5.0 TB/s).
+// N = 16384, four limbs: 2.2 GB in 0.441 ms, 5.0 TB/s).
 __global__ __launch_bounds__(256) void rope_kernel(DevCtx c, RopeArgs a, u32 n_blocks, u32 parts, u64 per) {
   u32 b = blockIdx.x;
   const u32 nb = b % n_blocks;
