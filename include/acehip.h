@@ -350,8 +350,10 @@ int acehip_bsgs_inner_rot(acehip_ctx* ctx, uint64_t* const* d_out0, uint64_t* co
  *
  * A matrix of ciphertexts, strides in words: polynomial `comp` of element (head, row, col) starts at data + head*head_stride + row*row_stride
  * + col*col_stride + comp*comp_stride.  The strides of an operand are arbitrary (0: the same for all); the polynomials of a result must not
- * overlap each other or an operand, unless an entry point says so.  Of every polynomial only the limbs of the call are touched.  Counts of
- * zero are allowed: an empty result is nothing to do, an empty sum is zero.
+ * overlap each other or an operand, unless an entry point says so; they may lie among each other, and among the polynomials of operands, in any way
+ * (where strides cross so often that 2^20 polynomials do not tell, the call is refused).  Of every polynomial only the limbs of the call are touched.
+ * Counts of zero are allowed: an empty result is nothing to do, an empty sum is zero.  A call whose launch would need 2^32 lanes is refused: of
+ * acehip_linear_i8 rows * n_comp * n_out results from 2^35 / N on, of acehip_rope rows * dim / 2 pairs from 2^32 / N on (in rings from 256 on).
  * Integer factors (`int64_t`, device arrays, shared by all limbs) are taken mod each prime: llround(factor * scaling_factor) is the usual value.
  * Data, weights and factors are read when the launch runs; arrays named h_* are read during the call.  Under a replica selection, operands in the
  * arena follow their replica, and the result has to lie in the arena; a sharded context computes the limbs that it owns. */
